@@ -67,10 +67,10 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def _build_host(verbose: bool) -> None:
-    """The Python module with the host path (``csrc/host.cpp``), against torch's C++ headers and the
+    """The Python module with the host path (``csrc/host*.cpp``), against torch's C++ headers and the
     library next to it.  Rebuilt when its sources, the command, torch or the interpreter have changed."""
-    src = CSRC / "host.cpp"
-    newest = max(src.stat().st_mtime, (INCLUDE / "fa2_b200.h").stat().st_mtime)
+    sources = sorted(CSRC.glob("host*.cpp"))
+    newest = max(f.stat().st_mtime for f in [*sources, CSRC / "host.h", INCLUDE / "fa2_b200.h"])
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -79,7 +79,7 @@ def _build_host(verbose: bool) -> None:
                 sysconfig.get_paths()["include"], cuda / "include"]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{p}" for p in includes), str(src), "-o", str(HOST_PATH),
+           *(f"-I{p}" for p in includes), *map(str, sources), "-o", str(HOST_PATH),
            f"-L{PKG_DIR}", f"-l:{LIB_PATH.name}", "-Wl,-rpath,$ORIGIN", f"-L{root / 'lib'}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]  # already loaded by `import torch`
     key = "\n".join([torch.__version__, sys.version, *cmd])
@@ -89,10 +89,10 @@ def _build_host(verbose: bool) -> None:
         return
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stderr[-4000:]}")
+        raise RuntimeError(f"g++ failed for the host module:\n{res.stderr[-4000:]}")
     stamp.write_text(key)
     if verbose:
-        print(f"[build] compiled {src.name}")
+        print(f"[build] compiled {HOST_PATH.name}")
 
 
 def build(verbose: bool = True, force: bool = False) -> Path:

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/fa2_b200.h"
+#include "capi.cuh"
 #include "common.cuh"
 
 namespace fa2 {
@@ -163,6 +164,17 @@ void make_ctx(DeviceState* d, LaunchCtx* ctx) {
   ctx->num_sms = d->num_sms;
 }
 
+}  // namespace
+
+int launch_context(LaunchCtx* ctx) {
+  DeviceState* d = nullptr;
+  if (int e = device_state(&d)) return e;
+  make_ctx(d, ctx);
+  return FA2_OK;
+}
+
+namespace {
+
 int check_shape(int B, int H, int N, int D, int dtype) {
   if (D < 8 || D > 256 || D % 8 != 0) return FA2_ERR_HEAD_DIM;
   if (dtype != FA2_DTYPE_FP16 && dtype != FA2_DTYPE_BF16) return FA2_ERR_DTYPE;
@@ -222,13 +234,17 @@ const char* fa2_strerror(int code) {
     case FA2_ERR_MISALIGNED: return "tensor pointers must be 16-byte aligned, fp32 outputs 32-byte aligned";
     case FA2_ERR_SHAPE: return "B, H, N must be positive, B*H <= 65535, N <= 2^24, 1 <= Nk <= N";
     case FA2_ERR_ARCH: return "the current device is not compute capability 10.x (B200)";
-    case FA2_ERR_DEVICE_STATUS: return "a kernel abandoned a bounded wait (see fa2_device_status)";
+    case FA2_ERR_DEVICE_STATUS:
+      return "a kernel abandoned a bounded wait, or met a page or position outside the cache (see fa2_device_status)";
     case FA2_ERR_DRIVER: return "cuTensorMapEncodeTiled is unavailable or rejected the tensor";
     case FA2_ERR_SCALE: return "softmax scale must be finite and > 0";
     case FA2_ERR_WORKSPACE:
       return "this backward mode needs a workspace of at least its minimum size (fa2_bwd_workspace_bytes)";
     case FA2_ERR_STRIDE:
       return "strides must be positive multiples of 8 elements (16 bytes), row stride >= D";
+    case FA2_ERR_HEADS: return "the query heads must be a multiple of the key and value heads";
+    case FA2_ERR_ROTARY:
+      return "the rotated columns must be a multiple of 16 up to the head dimension, with both tables given";
     case FA2_ERR_TOO_LARGE: return "problem exceeds the built-in scratch (B*H*ceil(N/128) > 4096)";
     default: break;
   }

@@ -26,7 +26,25 @@
 #include <cstring>
 #include <exception>
 
-#include "../../include/fa2_b200.h"
+#include "host.h"
+
+namespace fa2_host {
+void check_code(const char* fn, int code) {
+  if (code == 0) return;
+  pybind11::gil_scoped_acquire gil;
+  try {
+    pybind11::module_::import("flash_attention_triton_b200._lib").attr("check")(fn, code);
+  } catch (pybind11::error_already_set& e) {
+    e.restore();
+    python_error error;
+    error.persist();
+    throw error;
+  }
+}
+}  // namespace fa2_host
+
+using fa2_host::check_code;
+using fa2_host::dtype_code;
 
 namespace {
 
@@ -49,8 +67,6 @@ struct StrideArray {
       for (int d = 0; d < 3; ++d) v[3 * i + d] = ts[i]->stride(d);
   }
 };
-
-int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FA2_DTYPE_FP16 : FA2_DTYPE_BF16; }
 
 bool tensors(PyObject* const* args, int n) {
   for (int i = 0; i < n; ++i)
@@ -205,27 +221,12 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // forward and backward 112 -> 76 (52 of them torch's engine and an empty function), forward alone 17.6 -> 7.3.
 // ---------------------------------------------------------------------------------------------------------
 constexpr const char* kApiModule = "flash_attention_triton_b200.api";
-constexpr const char* kLibModule = "flash_attention_triton_b200._lib";
 
 // Environment switches that api.py serves.  Called with the interpreter lock, under which os.environ changes them.
 bool python_path_asked() {
   const char* check = std::getenv("FA2_B200_CHECK_STATUS");
   const char* mode = std::getenv("FA2_B200_BWD_MODE");
   return (check && std::strcmp(check, "1") == 0) || (mode && *mode);
-}
-
-// Raises _lib.Fa2Error for a non-zero code.  Called without the interpreter lock.
-void check_code(const char* fn, int code) {
-  if (code == 0) return;
-  pybind11::gil_scoped_acquire gil;
-  try {
-    pybind11::module_::import(kLibModule).attr("check")(fn, code);
-  } catch (pybind11::error_already_set& e) {
-    e.restore();
-    python_error error;
-    error.persist();
-    throw error;
-  }
 }
 
 constexpr int kModeAtomic = 0, kModeRecompute = 1, kModeSpill = 2;
@@ -450,6 +451,8 @@ PyMethodDef kMethods[] = {
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(backward)), METH_FASTCALL, nullptr},
     {"backward_mode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_backward_mode)), METH_FASTCALL, nullptr},
     {"allocate_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_allocate_workspace)), METH_FASTCALL, nullptr},
+    {"kv_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fa2_host::kv_append)), METH_FASTCALL, nullptr},
+    {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fa2_host::decode)), METH_FASTCALL, nullptr},
     {"readable_in_place", is_readable_in_place, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,52 @@
+// What the files of the Python module `_host` share.
+#pragma once
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
+
+#include "../../include/fa2_b200.h"
+
+namespace fa2_host {
+
+// Raises _lib.Fa2Error for a non-zero code.  Called without the interpreter lock.
+void check_code(const char* fn, int code);
+
+inline int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FA2_DTYPE_FP16 : FA2_DTYPE_BF16; }
+inline bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+
+// A tensor argument, or an undefined one for None where that is allowed; TypeError for anything else.
+inline at::Tensor tensor_argument(PyObject* arg, const char* name, bool optional = false) {
+  if (optional && arg == Py_None) return {};
+  TORCH_CHECK_TYPE(THPVariable_Check(arg), name, " must be a tensor", optional ? " or None" : "");
+  const at::Tensor& t = THPVariable_Unpack(arg);
+  TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided, name, " must be a dense tensor");
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
+// The softmax scale of a call: None and 0.0 mean 1 / sqrt(head dim).
+inline double scale_argument(PyObject* arg, int64_t head_dim) {
+  const double scale = arg == Py_None ? 0.0 : PyFloat_AsDouble(arg);
+  if (scale == -1.0 && PyErr_Occurred()) throw python_error();
+  return scale == 0.0 ? 1.0 / std::sqrt(static_cast<double>(head_dim)) : scale;
+}
+
+// Kernels read a [rows, H, D] tensor through its own strides: unit last stride, 16-byte aligned base, row and head
+// strides that are multiples of 8 elements and at least D (those of dimensions of size 1 do not matter).
+bool rows_readable(const at::Tensor& t);
+inline at::Tensor rows_input(const at::Tensor& t) { return rows_readable(t) ? t : t.contiguous(); }
+
+// AssertionError as flash_attention_v2 raises it, for what is not a CUDA tensor; ValueError for another device.
+void check_devices(std::initializer_list<std::pair<const at::Tensor*, const char*>> tensors);
+
+PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs);
+PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t nargs);
+
+}  // namespace fa2_host

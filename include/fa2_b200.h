@@ -52,6 +52,8 @@ extern "C" {
 #define FA2_ERR_WORKSPACE (-10)        /* the mode needs a workspace: NULL, or smaller than its minimum */
 #define FA2_ERR_TOO_LARGE (-11)        /* fa2_bwd_static_scratch: B*H*ceil(N/128) > 4096 */
 #define FA2_ERR_STRIDE (-12)           /* a stride is <= 0, not a multiple of 8 elements, or row < D */
+#define FA2_ERR_HEADS (-13)            /* Hq is not a multiple of Hkv */
+#define FA2_ERR_ROTARY (-14)           /* rotary not a multiple of 16 in [0, D], or a table missing */
 
 /* Opaque stream handle: pass a cudaStream_t (NULL = legacy default stream). */
 typedef void* fa2_stream_t;
@@ -256,6 +258,49 @@ int fa2_bwd_static_scratch(const void* q, const void* k, const void* v, const vo
                            const void* dout, const float* lse, void* dq, void* dk, void* dv,
                            int B, int H, int N, int D, int dtype, float scale,
                            fa2_stream_t stream);
+
+/*
+ * A paged key-value cache, which the reference does not have: k_cache and v_cache are 16-bit tensors
+ * [pages, page_size, Hkv, D], and page block_table[s][p / page_size] holds position p of sequence s in its
+ * slot p % page_size.  block_table is int32 [batch, table_width], lengths int32 [batch]: how many positions of a
+ * sequence the cache holds, THOSE THAT THIS CALL APPENDS INCLUDED, so that one tensor serves fa2_kv_append and
+ * the fa2_decode after it, in every layer.  A length of 0 marks an empty place of the batch.  Kernels read
+ * all three on the device.
+ *
+ * A page number outside [0, pages), or a position beyond the block table or the rotation tables, is not
+ * followed: fa2_kv_append leaves that token out, fa2_decode leaves those keys out, and both set the status word
+ * (fa2_device_status reports 0x40000 | 1 and 0x40000 | 2).
+ */
+
+/*
+ * Appends the keys and values of `tokens` new tokens, k and v [tokens, Hkv, D], and rotates on the way.
+ * cu_seqlens (int32 [batch + 1]) says which rows are whose: rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 are the
+ * last positions of sequence s.  NULL: one token a sequence, tokens == batch.  Row i of sequence s has position
+ * p = lengths[s] - (its rows) + i; a token of a negative position is not written.  Two tokens of a call must not
+ * have the same slot.
+ * rotary: the first `rotary` columns of every key are rotated by position (0: none): columns (j, j + rotary / 2),
+ * or (2 j, 2 j + 1) with `interleaved`, by the angle whose cosine and sine are cos[p][j] and sin[p][j], fp32
+ * [positions, rotary / 2].  fp32 arithmetic, rounded once.
+ * q [tokens, Hq, D] (or NULL) is rotated by the same positions into q_out; k_out (or NULL) gets the rotated
+ * keys as well.  Both are dense; their rows of tokens that are not written, and rows behind the last sequence, are zeros.
+ * strides (elements): q, k, v (row, head), k_cache, v_cache (page, slot, head), block_table (row), 13 values; NULL: dense.
+ */
+int fa2_kv_append(const void* q, const void* k, const void* v, void* q_out, void* k_out, void* k_cache, void* v_cache,
+                  const int* block_table, const int* lengths, const int* cu_seqlens, const float* cos, const float* sin,
+                  int tokens, int batch, int Hq, int Hkv, int D, int pages, int page_size, int table_width, int positions,
+                  int rotary, int interleaved, int dtype, const long long* strides, fa2_stream_t stream);
+
+/*
+ * out[s, h] = softmax(scale * q[s, h] K^T) V over the first lengths[s] positions of sequence s, with the keys and values of
+ * head h * Hkv / Hq; zeros where lengths[s] <= 0.  q [batch, Hq, D], out dense [batch, Hq, D].  The cache is cut over all SMs
+ * whatever the lengths are; `workspace` (16-byte aligned, fa2_decode_workspace_bytes) holds the parts that are joined in
+ * a fixed order, so the same call gives the same bits.
+ * strides (elements): q (row, head), k_cache, v_cache (page, slot, head), block_table (row), 9 values; NULL: dense.
+ */
+int fa2_decode(const void* q, const void* k_cache, const void* v_cache, void* out, const int* block_table,
+               const int* lengths, void* workspace, size_t workspace_bytes, int batch, int Hq, int Hkv, int D, int pages,
+               int page_size, int table_width, int dtype, float scale, const long long* strides, fa2_stream_t stream);
+size_t fa2_decode_workspace_bytes(int batch, int Hq, int Hkv, int D, int page_size, int table_width);
 
 #ifdef __cplusplus
 }
