@@ -1,7 +1,7 @@
 """B200-native (sm_100a) causal FlashAttention-2 with the public surface of flash-attention-triton.
 
 Exports the same four names as the reference package (``src/flash_attention_triton/__init__.py:13``)
-plus the autograd function, and what the reference has no counterpart of: the paged key-value cache.
+plus the autograd function, and what the reference has no counterpart of: packed sequences with grouped heads, and the paged key-value cache.
 """
 
 from .api import (
@@ -11,6 +11,7 @@ from .api import (
     flash_attention_v2_custom,
     init_to_zero_v2,
 )
+from .packed import flash_attention_packed
 from .paged import append_kv_cache, flash_attention_decode, rotary_tables
 from .partition import shard_range, shard_slab
 
@@ -21,6 +22,7 @@ __all__ = [
     "KernelsConfigV2",
     "append_kv_cache",
     "flash_attention_decode",
+    "flash_attention_packed",
     "flash_attention_v2",
     "flash_attention_v2_custom",
     "init_to_zero_v2",

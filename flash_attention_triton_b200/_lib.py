@@ -39,6 +39,10 @@ SYMBOLS = [
     ("fa2_fwd_strided_f32", c_int, [c_void_p] * 6 + [c_int] * 6 + [c_float, c_void_p, c_void_p]),
     ("fa2_bwd_strided_f32", c_int,
      [c_void_p] * 9 + [c_size_t] + [c_int] * 6 + [c_float, c_int, c_void_p, c_void_p]),
+    ("fa2_packed_plan_bytes", c_size_t, [c_int] * 2),
+    ("fa2_packed_fwd", c_int, [c_void_p] * 7 + [c_int] * 6 + [c_float, c_void_p, c_void_p]),
+    ("fa2_packed_bwd_workspace_bytes", c_size_t, [c_int] * 3),
+    ("fa2_packed_bwd", c_int, [c_void_p] * 12 + [c_size_t] + [c_int] * 6 + [c_float, c_void_p, c_void_p]),
     ("fa2_kv_append", c_int, [c_void_p] * 12 + [c_int] * 12 + [c_void_p, c_void_p]),
     ("fa2_decode", c_int, [c_void_p] * 7 + [c_size_t] + [c_int] * 8 + [c_float, c_void_p, c_void_p]),
     ("fa2_decode_workspace_bytes", c_size_t, [c_int] * 6),

@@ -134,15 +134,16 @@ int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N,
   return r == CUDA_SUCCESS ? FA2_OK : FA2_ERR_DRIVER;
 }
 
-// Tensor map over a [B, H, N, D] 16-bit tensor with box (chunk, box_rows, 1, 1).  The chunk
-// follows the padded head dim, so for D = 48 or 96 the last box of a row hangs over the
-// tensor: those columns read as zeros and are not written.
+}  // namespace
+
 int make_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D,
              const Strides& st, int box_rows) {
   const int chunk = padded_head_dim(D) >= 64 ? 64 : 32;
   return encode_map(m, base, dtype, B, H, N, D, st, chunk, box_rows,
                     chunk == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }

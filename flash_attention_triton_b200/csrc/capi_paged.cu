@@ -6,13 +6,6 @@
 #include "paged.cuh"
 
 namespace fa2 {
-namespace {
-
-// Strides of a tensor whose last dimension has `last` elements: positive multiples of 8 where the dimension has more
-// than one entry; rows of heads and slots must not overlap.
-bool stride_ok(long long stride, int size, int last) {
-  return size <= 1 || (stride >= last && stride % 8 == 0 && stride < (1ll << 38));
-}
 
 int check_heads(int Hq, int Hkv, int D, int dtype) {
   if (D < 8 || D > 256 || D % 8 != 0) return FA2_ERR_HEAD_DIM;
@@ -20,6 +13,8 @@ int check_heads(int Hq, int Hkv, int D, int dtype) {
   if (Hkv < 1 || Hq < 1 || Hq > 65535) return FA2_ERR_SHAPE;
   return Hq % Hkv ? FA2_ERR_HEADS : FA2_OK;
 }
+
+namespace {
 
 int check_cache(int batch, int pages, int page_size, int table_width) {
   if (batch < 1 || batch > (1 << 20) || pages < 1 || page_size < 1 || table_width < 1) return FA2_ERR_SHAPE;

@@ -451,6 +451,7 @@ PyMethodDef kMethods[] = {
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(backward)), METH_FASTCALL, nullptr},
     {"backward_mode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_backward_mode)), METH_FASTCALL, nullptr},
     {"allocate_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_allocate_workspace)), METH_FASTCALL, nullptr},
+    {"packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fa2_host::packed)), METH_FASTCALL, nullptr},
     {"kv_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fa2_host::kv_append)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(fa2_host::decode)), METH_FASTCALL, nullptr},
     {"readable_in_place", is_readable_in_place, METH_O, nullptr},

@@ -46,6 +46,9 @@ inline at::Tensor rows_input(const at::Tensor& t) { return rows_readable(t) ? t 
 // AssertionError as flash_attention_v2 raises it, for what is not a CUDA tensor; ValueError for another device.
 void check_devices(std::initializer_list<std::pair<const at::Tensor*, const char*>> tensors);
 
+void check_int32(const at::Tensor& t, const char* name, int dims);  // contiguous in its last dimension
+
+PyObject* packed(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t nargs);
 

@@ -10,6 +10,11 @@ bool rows_readable(const at::Tensor& t) {
   return true;
 }
 
+void check_int32(const at::Tensor& t, const char* name, int dims) {
+  TORCH_CHECK_VALUE(t.dim() == dims && t.scalar_type() == at::kInt, name, dims == 1 ? " must be an int32 tensor of one dimension" : " must be an int32 tensor of two dimensions");
+  TORCH_CHECK_VALUE(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
+}
+
 void check_devices(std::initializer_list<std::pair<const at::Tensor*, const char*>> tensors) {
   const at::Tensor* first = nullptr;
   for (const auto& [t, name] : tensors) {
@@ -25,11 +30,6 @@ void check_devices(std::initializer_list<std::pair<const at::Tensor*, const char
 }
 
 namespace {
-
-void check_int32(const at::Tensor& t, const char* name, int dims) {
-  TORCH_CHECK_VALUE(t.dim() == dims && t.scalar_type() == at::kInt, name, dims == 1 ? " must be an int32 tensor of one dimension" : " must be an int32 tensor of two dimensions");
-  TORCH_CHECK_VALUE(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, name, " must be contiguous in its last dimension");
-}
 
 struct Cache {
   int batch, pages, page_size, table_width, Hkv, D;

@@ -1,0 +1,104 @@
+// Attention over packed sequences: sequences of different lengths one behind the other in [rows, heads, D] tensors,
+// cu_seqlens[s] .. cu_seqlens[s + 1] - 1 the rows of sequence s, and G = Hq / Hkv query heads to a key head.
+//
+// The kernels work on 128-row tiles of the sequences.  Which tiles there are only the device knows, so a kernel in
+// front of them writes the plan: every tile of every sequence, the ones that meet the most tiles first, for the same reason
+// as grouped_order in common.cuh.  Tile t of a sequence of n tiles meets t + 1 KV tiles as a Q tile; KV tile n - 1 - t
+// meets as many Q tiles, so one order serves both.
+//
+// What the tensor maps cannot know either is where a sequence ends inside a tile.  Loads bring the rows of the next
+// sequence along (or zeros behind the last row): as rows of the result they are not stored, and where they are
+// summed over (V; Q and dO for dK and dV; K and V for dQ) the warp that issues the product first clears them in
+// shared memory, because 0 x NaN is none.  Stores of 32 rows go through the tensor map where all of them belong
+// to the sequence, row by row where not.
+#pragma once
+#include "common.cuh"
+#include "paged.cuh"
+#include "ptx.cuh"
+
+namespace fa2 {
+
+// One tile, or two adjacent ones, of a sequence.
+struct PackedTile {
+  int row0;    // first row of the sequence
+  int length;  // its rows
+  int tile;    // (first) tile of this entry
+  int base;    // number of the sequence's tile 0 among all tiles, in the order of the sequences
+};
+
+struct PackedPlan {
+  int* counts;         // [0] tiles, [1] pairs of tiles
+  PackedTile* tiles;   // heaviest first, room for `capacity`
+  PackedTile* pairs;   // pairs of adjacent tiles, likewise
+  int capacity;
+};
+// Tiles of `rows` rows in `batch` sequences, at most.
+inline int packed_capacity(int rows, int batch) { return rows / 128 + batch; }
+inline size_t packed_plan_bytes(int rows, int batch) { return 16 + 2 * sizeof(PackedTile) * packed_capacity(rows, batch); }
+inline PackedPlan packed_plan(void* p, int rows, int batch) {
+  const int n = packed_capacity(rows, batch);
+  PackedTile* const tiles = reinterpret_cast<PackedTile*>(static_cast<char*>(p) + 16);
+  return PackedPlan{static_cast<int*>(p), tiles, tiles + n, n};
+}
+
+struct PackedShape {
+  int rows, batch, Hq, Hkv;
+  int D;   // head dim the kernels are instantiated for: 32, 64 or 128
+  int Dg;  // of the tensors
+  int dtype;
+  float scale;
+};
+
+// What the backward's preprocess leaves: -lse log2(e) and -delta by tile, [Hq][capacity][2][128], rows behind a
+// sequence -inf and 0; at fp16 also the largest |dout| of every 32 rows, [Hkv][capacity][4][G] (see head_dscale).
+struct PackedStats {
+  float* stats;
+  unsigned* amax;
+};
+inline size_t packed_stats_bytes(int rows, int batch, int Hq) {
+  return static_cast<size_t>(packed_capacity(rows, batch)) * Hq * (256 + 4) * 4;
+}
+
+// Status word of cu_seqlens that fall, or leave the rows: every output is zero then.
+constexpr int kStatusSequences = 0x80000;
+
+cudaError_t launch_packed_plan(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, bool pairs, void* out,
+                               int* status, int num_sms, cudaStream_t stream);
+cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                              const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, const LaunchCtx& ctx,
+                              cudaStream_t stream);
+cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& plan, const int* cu_seqlens, const void* o,
+                                     const void* dout, const RowStrides& sdo, const float* lse, const PackedStats& stats,
+                                     void* dq, void* dk, void* dv, cudaStream_t stream);
+// Rows of a step of the backward kernels, and the box height of the tensors they walk.
+int packed_step_rows(const PackedShape& s, int num_sms);
+cudaError_t launch_packed_dkdv(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                               const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
+                               void* dk, void* dv, const PackedStats& stats, int step_rows, int* status, cudaStream_t stream);
+cudaError_t launch_packed_dq(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                             const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdq, void* dq,
+                             const PackedStats& stats, int step_rows, int* status, cudaStream_t stream);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
+  const uint4 v = ld_global(reinterpret_cast<const uint4*>(p));
+  return PackedTile{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w)};
+}
+
+// Clears rows `first` .. ROWS - 1 of a staged [ROWS, D] tile (whole warp; nothing where first >= ROWS) before a product sums
+// over them.  A row stays within its own bytes under the swizzle, so the end of every chunk tile is cleared as it lies.
+template <int D, int ROWS>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int first, int lane) {
+  using T = Tile<D>;
+  if (first >= ROWS) return;
+  if (first < 0) first = 0;
+  __syncwarp();
+  for (int ch = 0; ch < T::kChunks; ++ch)
+    for (int at = first * T::kRowBytes + lane * 16; at < ROWS * T::kRowBytes; at += 512)
+      *reinterpret_cast<uint4*>(tile + ch * (ROWS * T::kRowBytes) + at) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+#endif
+
+}  // namespace fa2

@@ -260,6 +260,31 @@ int fa2_bwd_static_scratch(const void* q, const void* k, const void* v, const vo
                            fa2_stream_t stream);
 
 /*
+ * Causal attention over packed sequences of different lengths with grouped heads, which the reference does not have.
+ * q, o, dout, dq are [rows, Hq, D], k, v, dk, dv [rows, Hkv, D] with Hkv dividing Hq (query head h goes with key head
+ * h * Hkv / Hq), D a multiple of 8 up to 128.  Rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [batch + 1], read on
+ * the device) are sequence s; every row sees the rows of its own sequence up to itself.  Rows of no sequence get
+ * zeros in o, dq, dk and dv, and are never read into another row's result.  cu_seqlens that fall or leave [0, rows] set the status
+ * word (0x80000), and every output is zero.
+ * fa2_packed_fwd writes the order in which the kernels take the tiles of the sequences into `plan` (16-byte aligned,
+ * fa2_packed_plan_bytes), which fa2_packed_bwd reads, and lse, fp32 [Hq, rows] (natural log; rows of no sequence are left
+ * alone).  The work counter of fa2_fwd's note on captured calls is used here too: replays of one graph must not overlap.
+ * fa2_packed_bwd recomputes the scores for dK / dV and for dQ, so it needs no memory beyond O(rows): `workspace`
+ * (16-byte aligned, fa2_packed_bwd_workspace_bytes) holds the row statistics.  dk and dv are summed over the query heads
+ * of a key head in 32 bits; every sum has one owner and one order, so the same call gives the same bits.
+ * strides (elements, row and head of each): q, k, v (6 values), backward q, k, v, dout (8 values); NULL: dense.  o, dq, dk, dv are dense.
+ */
+size_t fa2_packed_plan_bytes(int rows, int batch);
+int fa2_packed_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu_seqlens, void* plan,
+                   int rows, int batch, int Hq, int Hkv, int D, int dtype, float scale, const long long* strides,
+                   fa2_stream_t stream);
+size_t fa2_packed_bwd_workspace_bytes(int rows, int batch, int Hq);
+int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, void* dq,
+                   void* dk, void* dv, const int* cu_seqlens, const void* plan, void* workspace, size_t workspace_bytes,
+                   int rows, int batch, int Hq, int Hkv, int D, int dtype, float scale, const long long* strides,
+                   fa2_stream_t stream);
+
+/*
  * A paged key-value cache, which the reference does not have: k_cache and v_cache are 16-bit tensors
  * [pages, page_size, Hkv, D], and page block_table[s][p / page_size] holds position p of sequence s in its
  * slot p % page_size.  block_table is int32 [batch, table_width], lengths int32 [batch]: how many positions of a
