@@ -135,14 +135,22 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
   else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
-__device__ __forceinline__ uint16_t to_16bit(float x, bool bf16) {
-  return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+// What a part with maximum m and sum l counts beside the maximum `top` of all of them.  A part without a finite score has
+// l = 0, or NaN where a score was NaN.
+__device__ __forceinline__ float part_weight(float m, float l, float top, float scale_log2) {
+  return m == -INFINITY ? l * 0.f : ex2((m - top) * scale_log2);
 }
 
-// Partial results in the workspace: CTA c has two places, 2 c for the part that continues what the CTA before began
-// and 2 c + 1 for the one that it begins; a place is m, l of `rows` rows and their o.
-__device__ __forceinline__ float* partial(float* workspace, int place, int rows, int D) {
-  return workspace + static_cast<long long>(place) * rows * (D + 2);
+// The workspace: for each CTA what it has begun and not ended, then the partial results.  CTA c has two places for those,
+// 2 c for the part that continues what the CTA before began and 2 c + 1 for the one that it begins; a place is m, l of
+// `rows` rows and their o.
+struct Cut {
+  int b, h;  // as in Walk
+  int last;  // CTA that has the last unit; below 0: it has ended what it began
+  int units; // of the CTA's stretch
+};
+__device__ __forceinline__ float* partial(float* workspace, int ctas, int place, int rows, int D) {
+  return workspace + ctas * 4 + static_cast<long long>(place) * rows * (D + 2);
 }
 
 template <int DP, bool BF16>
@@ -176,7 +184,11 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   const long long total = units_before(a, a.batch, lane) * heads;
   const long long u0 = stretch_start(total, blockIdx.x, gridDim.x);
   const int count = static_cast<int>(stretch_start(total, blockIdx.x + 1, gridDim.x) - u0);
-  if (count == 0) return;
+  Cut* const cut = reinterpret_cast<Cut*>(a.workspace) + blockIdx.x;
+  if (count == 0) {
+    if (threadIdx.x == 0) *reinterpret_cast<int4*>(cut) = make_int4(0, 0, -1, 0);
+    return;
+  }
   Walk load;
   find_unit(a, heads, u0, lane, load);
   Walk work = load;
@@ -341,7 +353,13 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     if (ends || n + 1 == count) {
       const bool begins = work.unit <= n;  // its first unit is in this stretch
       const bool whole = begins && ends;
-      float* const part = partial(a.workspace, 2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
+      float* const part = partial(a.workspace, gridDim.x, 2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
+      if (n + 1 == count && threadIdx.x == 0) {
+        // the CTA of a unit is the last one whose stretch starts at or before it
+        const long long last = u0 + n + (work.units - 1 - work.unit);
+        const int cta = begins && !ends ? static_cast<int>(((last + 1) * gridDim.x - 1) / total) : -1;
+        *reinterpret_cast<int4*>(cut) = make_int4(work.b, work.h, cta, count);
+      }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         if (r * kJoinRows >= here) break;
@@ -367,11 +385,12 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
           float all = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float f = mw[w] == -INFINITY ? 0.f : ex2((mw[w] - top) * a.scale_log2);
+            const float lw = join_ml[(w * kJoinRows + row) * 2 + 1];
+            const float f = part_weight(mw[w], lw, top, a.scale_log2);
             const float2 x = *reinterpret_cast<const float2*>(join + (w * kJoinRows + row) * C::kJoinStride + col);
             sum.x = fmaf(f, x.x, sum.x);
             sum.y = fmaf(f, x.y, sum.y);
-            all = fmaf(f, join_ml[(w * kJoinRows + row) * 2 + 1], all);
+            all = fmaf(f, lw, all);
           }
           if (whole) {
             const float inv = 1.f / all;
@@ -390,38 +409,79 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   }
 }
 
-// Adds up the parts of the (sequence, key head)s that decode_kernel's stretches cut apart; one CTA for each query head.
+// Adds up the parts of what decode_kernel's stretches cut apart: block (c, row) one query head of what CTA c began and did
+// not end.  First the weights of all parts, one a thread, then the parts, D / 2 threads to each, so that no load waits for
+// another.  Few long sequences have a hundred parts and more to a head: one thread a column, part after part, took
+// 73 us on two sequences of 131072 keys.
+constexpr int kJoinThreads = 256;
 template <bool BF16>
-__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int ctas) {
-  const int lane = threadIdx.x & 31;
-  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
-  const int heads = a.Hkv * blocks;
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq;
-  const int h = hq / group * blocks + hq % group / kRows, row = hq % group % kRows;
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int ctas) {
+  __shared__ float weight[kJoinThreads], reduced[kJoinThreads / 32];
+  __shared__ float2 sums[kJoinThreads];
   grid_wait_previous();
   grid_allow_next();
-  const int units = units_of(clamp_length(a, b));
-  if (units == 0) return;
-  const long long before = units_before(a, b, lane);
-  const long long total = (before + units_before(a, a.batch, lane) - before) * heads;
-  const long long first = before * heads + static_cast<long long>(h) * units, last = first + units - 1;
-  // the CTA of a unit: the last one whose stretch starts at or before it
-  const int c0 = static_cast<int>(((first + 1) * ctas - 1) / total), c1 = static_cast<int>(((last + 1) * ctas - 1) / total);
-  if (c0 == c1) return;  // one CTA had all of it and wrote the result
-  for (int col = threadIdx.x; col < a.D; col += 128) {
-    float top = -INFINITY, all = 0.f, sum = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      if (stretch_start(total, c, ctas) == stretch_start(total, c + 1, ctas)) continue;
-      const float* const part = partial(a.workspace, 2 * c + (c == c0 ? 1 : 0), rows, a.D);
-      const float mc = ld_global(part + 2 * row), lc = ld_global(part + 2 * row + 1), x = ld_global(part + 2 * rows + row * a.D + col);
-      if (mc == -INFINITY) continue;
-      const float now = fmaxf(top, mc);
-      const float f = top == -INFINITY ? 0.f : ex2((top - now) * a.scale_log2), g = ex2((mc - now) * a.scale_log2);
-      all = all * f + lc * g;
-      sum = sum * f + x * g;
-      top = now;
+  const int c0 = blockIdx.x / rows, row = blockIdx.x - c0 * rows;
+  const uint4* const cuts = reinterpret_cast<const uint4*>(a.workspace);
+  const uint4 cut = ld_global(cuts + c0);  // a Cut
+  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
+  const int h = static_cast<int>(cut.y), kv_head = h / blocks, in_group = (h - kv_head * blocks) * kRows + row;
+  if (static_cast<int>(cut.z) < 0 || in_group >= group) return;
+  const int parts = static_cast<int>(cut.z) - c0 + 1, d2 = a.D / 2;
+  const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = kJoinThreads / d2;
+  auto part = [&](int i) { return partial(a.workspace, ctas, 2 * (c0 + i) + (i == 0 ? 1 : 0), rows, a.D); };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top = -INFINITY, all = 0.f;
+  float2 sum = make_float2(0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += kJoinThreads) {
+    const int here = min(parts - p0, kJoinThreads);
+    float m = -INFINITY, l = 0.f;
+    // a CTA without units (there are fewer units than CTAs) has left nothing
+    if (threadIdx.x < here && ld_global(cuts + c0 + p0 + threadIdx.x).w != 0) {
+      const float* const at = part(p0 + threadIdx.x) + 2 * row;
+      m = ld_global(at), l = ld_global(at + 1);
     }
-    static_cast<uint16_t*>(a.out)[(static_cast<long long>(b) * a.Hq + hq) * a.D + col] = to_16bit(sum / all, BF16);
+    float most = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) reduced[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) most = fmaxf(most, reduced[i]);
+    most = fmaxf(most, top);
+    const float old = part_weight(top, all, most, a.scale_log2);
+    all *= old, sum.x *= old, sum.y *= old;
+    top = most;
+    const float w = part_weight(m, l, top, a.scale_log2);
+    weight[threadIdx.x] = w;
+    l *= w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    __syncthreads();
+    if (lane == 0) reduced[warp] = l;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) all += reduced[i];
+    if (share < shares)
+#pragma unroll 4
+      for (int i = share; i < here; i += shares) {
+        const float f = weight[i];
+        if (f == 0.f) continue;
+        const float* const x = part(p0 + i) + 2 * rows + row * a.D + 2 * col;
+        sum.x = fmaf(f, ld_global(x), sum.x);
+        sum.y = fmaf(f, ld_global(x + 1), sum.y);
+      }
+    __syncthreads();
+  }
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (share == 0) {
+    for (int i = 1; i < shares; ++i) {
+      const float2 x = sums[i * d2 + col];
+      sum.x += x.x, sum.y += x.y;
+    }
+    const float inv = 1.f / all;  // NaN for a row without any finite score, as everywhere
+    uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.x) * a.Hq + kv_head * group + in_group) * a.D + 2 * col;
+    *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(sum.x * inv, sum.y * inv);
   }
 }
 
@@ -444,7 +504,7 @@ cudaError_t launch_decode_t(const DecodeArgs& a, int num_sms, int* status, cudaS
   const int ctas = decode_ctas(a, C::kCtasPerSm, num_sms);
   e = launch_dependent(kern, ctas, 32 * kWarps, C::kSmemBytes, stream, a, rows, status);
   if (e != cudaSuccess) return e;
-  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(a.batch) * a.Hq, 128, 0, stream, a, rows, ctas);
+  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(ctas) * rows, kJoinThreads, 0, stream, a, rows, ctas);
 }
 
 }  // namespace
@@ -453,7 +513,8 @@ size_t decode_workspace_floats(int batch, int Hq, int Hkv, int D, int table_widt
   const int group = Hq / Hkv, blocks = (group + kRows - 1) / kRows, rows = group < kRows ? group : kRows;
   const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit;
   const long long most = units * batch * Hkv * blocks;
-  return static_cast<size_t>(2 * (most < kMaxCtas ? most : kMaxCtas)) * rows * (D + 2);
+  const long long ctas = most < kMaxCtas ? most : kMaxCtas;
+  return static_cast<size_t>(ctas) * (4 + 2 * rows * (D + 2));
 }
 
 cudaError_t launch_decode(const DecodeArgs& a, int dtype, int num_sms, int* status, cudaStream_t stream) {

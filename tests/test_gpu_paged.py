@@ -340,3 +340,15 @@ def test_decode_on_the_other_device():
     want = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
     out = fa.flash_attention_decode(*(t.to("cuda:1") for t in (q, cache.k, cache.v, cache.table, cache.lengths())))
     assert torch.equal(out.cpu(), want.cpu())
+
+
+@pytest.mark.parametrize("where", [0, 63, 64, 2999])
+def test_decode_nan_reaches_the_output(where):
+    """A NaN key stays visible wherever its 16 keys end up among the parts that are joined, alone in them too."""
+    cache = Cache([3000, 65], [3000, 65], 16, 2, 64, BF16)
+    q = normal(2, 4, 64, dtype=BF16)
+    clean = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
+    cache.k[cache.places(0, [where])] = math.nan
+    cache.k[cache.places(1, [64])] = math.nan  # the only key of its 16
+    out = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
+    assert clean.isfinite().all() and out.isnan().all()

@@ -90,9 +90,9 @@ def test_head_dims(d):
 
 def test_workspace_size():
     lib = _lib.lib()
-    # two places for every CTA, no more CTAs than units of 64 keys; m, l and o of each row
-    assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 16, 4) == 2 * 2 * 4 * 66 * 4
-    assert lib.fa2_decode_workspace_bytes(1, 40, 2, 64, 16, 4) == 2 * 4 * 16 * 66 * 4  # 20 heads: two passes of 16 rows
+    # 16 bytes and two places for every CTA, no more CTAs than units of 64 keys; m, l and o of each row
+    assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 16, 4) == 2 * (16 + 2 * 4 * 66 * 4)
+    assert lib.fa2_decode_workspace_bytes(1, 40, 2, 64, 16, 4) == 4 * (16 + 2 * 16 * 66 * 4)  # 20 heads: two passes of 16 rows
     assert lib.fa2_decode_workspace_bytes(1, 3, 2, 64, 16, 4) == 0
     assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 1 << 16, 1 << 16) == 0
 
