@@ -116,6 +116,8 @@ int get_strides(const long long* user, int idx, int B, int H, int N, int D, Stri
   return FA2_OK;
 }
 
+}  // namespace
+
 int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D, const Strides& st,
                int box_columns, int box_rows, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn enc = get_encode();
@@ -133,8 +135,6 @@ int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N,
           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FA2_OK : FA2_ERR_DRIVER;
 }
-
-}  // namespace
 
 int make_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D,
              const Strides& st, int box_rows) {

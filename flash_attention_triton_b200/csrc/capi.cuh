@@ -10,7 +10,10 @@ namespace fa2 {
 // primary context to the calling thread.  Returns a code of fa2_b200.h or a cudaError_t.
 int launch_context(LaunchCtx* ctx);
 
-// Tensor map over a [B, H, N, D] 16-bit tensor with box (chunk, box_rows, 1, 1).  The chunk
+// Tensor map over a [B, H, N, D] 16-bit tensor with box (box_columns, box_rows, 1, 1).
+int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D, const Strides& st,
+               int box_columns, int box_rows, CUtensorMapSwizzle swizzle);
+// The same with box (chunk, box_rows, 1, 1).  The chunk
 // follows the padded head dim, so for D = 48 or 96 the last box of a row hangs over the
 // tensor: those columns read as zeros and are not written.
 int make_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D, const Strides& st, int box_rows);

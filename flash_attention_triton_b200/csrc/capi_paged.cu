@@ -98,7 +98,16 @@ int fa2_decode(const void* q, const void* k_cache, const void* v_cache, void* ou
     return FA2_ERR_STRIDE;
   LaunchCtx ctx;
   if (int e = launch_context(&ctx)) return e;
-  return static_cast<int>(launch_decode(a, dtype, ctx.num_sms, ctx.status, static_cast<cudaStream_t>(stream)));
+  CUtensorMap tk, tv;
+  const CacheStrides* const st[2] = {&a.sk_cache, &a.sv_cache};
+  for (int i = 0; i < 2; ++i) {
+    // strides of dimensions of size 1 carry no information
+    const long long slot = page_size > 1 ? st[i]->slot : D, head = Hkv > 1 ? st[i]->head : D, page = pages > 1 ? st[i]->page : D;
+    if (int e = encode_map(i ? &tv : &tk, i ? v_cache : k_cache, dtype, pages, Hkv, page_size, D, Strides{page, head, slot}, 64,
+                           decode_box_rows(page_size), CU_TENSOR_MAP_SWIZZLE_128B))
+      return e;
+  }
+  return static_cast<int>(launch_decode(tk, tv, a, dtype, ctx.num_sms, ctx.status, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -8,12 +8,13 @@
 // apart, each CTA leaves (m, l, o) of its part in the workspace, and decode_join_kernel adds the parts up in order:
 // the same bits every time.
 //
-// Inside a CTA warp w takes keys 16 w .. 16 w + 15 of every unit and runs on its own: its keys and values arrive
-// by 16-byte asynchronous copies in a ring of stages of its own, the query heads of the key head are the rows of
-// m16n8k16 products (S = Q K^T, O += P V, fp32 accumulators in registers), and maximum and sum of the softmax
-// run along.  The four warps meet where a (sequence, key head) ends, while their next stages are already loading.
-// The products cost a fifth of the time that the bytes take, so the mma.sync form does, and a row of
-// 16 queries needs no tile of 128.
+// Inside a CTA warp w takes keys 16 w .. 16 w + 15 of every unit and runs on its own: tiled copies bring its keys and
+// values into a ring of stages of its own, as many rows to a copy as 16 keys have next to each other in a page (16 where
+// the page size is a multiple of it).  The keys are the 16 rows of m16n8k16 products and the query heads of the key
+// head their 8 columns: S^T = K Q^T, O^T += V^T P^T, fp32 accumulators in registers, P^T turned around by
+// movmatrix.  Eight query heads fill the product; as its rows they would fill half of it.  The four warps meet
+// where a (sequence, key head) ends, while their next stages are already loading.  The products take a fraction of
+// the time that the bytes take, so mma.sync serves, and a row of eight queries needs no tile of 128.
 #include "common.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
@@ -23,18 +24,23 @@ namespace {
 
 constexpr int kUnit = 64;  // keys
 constexpr int kWarps = 4;
-constexpr int kRows = 16;  // query heads of a key head that one pass takes
-constexpr int kJoinRows = 8;  // rows that the warps of a CTA add up at a time
+constexpr int kJoinRows = 8;  // query heads that the warps of a CTA add up at a time
+// Query heads of a key head that one pass takes: 8 for each column tile of the products.
+inline int column_tiles(int group) { return group <= 8 ? 1 : 2; }
 constexpr int kMaxCtas = 1024;
 
 template <int DP>
 struct DecodeCfg {
   static constexpr int kStages = DP == 64 ? 4 : 3;
   static constexpr int kCtasPerSm = DP == 64 ? 3 : (DP == 128 ? 2 : 1);
-  static constexpr int kTileBytes = 16 * DP * 2;                           // 16 keys, or 16 values
+  static constexpr int kChunks = DP / 64;           // of 64 columns, what a box of a copy is wide
+  static constexpr int kTileBytes = 16 * DP * 2;    // 16 keys, or 16 values: [kChunks][16 rows][128 bytes], swizzled
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
-  static constexpr int kJoinStride = DP + 4;                               // floats of a row of partial sums
-  static constexpr int kSmemBytes = kWarps * kWarpBytes + kWarps * kJoinRows * (kJoinStride + 2) * 4;
+  static constexpr int kJoinStride = DP + 4;        // floats of a row of partial sums
+  static constexpr int kOffJoin = kWarps * kWarpBytes;
+  static constexpr int kOffBar = kOffJoin + kWarps * kJoinRows * (kJoinStride + 2) * 4;
+  static constexpr int kOffAbort = kOffBar + kWarps * kStages * 8;
+  static constexpr int kSmemBytes = kOffAbort + 16;
   static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of one SM");
 };
 
@@ -105,14 +111,6 @@ __device__ __forceinline__ void next_unit(const DecodeArgs& a, int heads, Walk& 
   } while (w.units == 0);
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -120,6 +118,11 @@ __device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void load_matrices_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <bool BF16>
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -153,25 +156,39 @@ __device__ __forceinline__ float* partial(float* workspace, int ctas, int place,
   return workspace + ctas * 4 + static_cast<long long>(place) * rows * (D + 2);
 }
 
-template <int DP, bool BF16>
+template <int DP, int NT, bool BF16>
 __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
-    decode_kernel(const __grid_constant__ DecodeArgs a, int rows, int* status) {
+    decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                  const __grid_constant__ DecodeArgs a, int rows, int box_rows, int* status) {
   using C = DecodeCfg<DP>;
-  constexpr int kPieces = DP / 8;  // 16-byte pieces of a row
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kRows = 8 * NT;
+  extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = smem_u32(smem) + warp * C::kWarpBytes;
-  float* const join = reinterpret_cast<float*>(smem + kWarps * C::kWarpBytes);  // [kWarps][kJoinRows][kJoinStride]
-  float* const join_ml = join + kWarps * kJoinRows * C::kJoinStride;            // [kWarps][kJoinRows][2]
+  const uint32_t base = smem_u32(smem);
+  if (base & 1023u) {  // swizzled tiles need 1024-byte alignment
+    if (threadIdx.x == 0) atomicCAS(status, 0, 0x20000 | kSiteDecode);
+    return;
+  }
+  const uint32_t ring = base + warp * C::kWarpBytes;
+  float* const join = reinterpret_cast<float*>(smem + C::kOffJoin);   // [kWarps][kJoinRows][kJoinStride]
+  float* const join_ml = join + kWarps * kJoinRows * C::kJoinStride;  // [kWarps][kJoinRows][2]
+  auto bar = [&](int stage) { return base + C::kOffBar + 8u * (warp * C::kStages + stage); };
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffAbort);
+  const WaitCtx w{abort_flag, status};
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
   const int heads = a.Hkv * blocks;
   const int d8 = a.D / 8;
 
-  // columns beyond the head dim are zeros that no copy touches
-  if (d8 < kPieces)
-    for (int i = lane; i < C::kWarpBytes / 16; i += 32)
-      *reinterpret_cast<uint4*>(smem + warp * C::kWarpBytes + i * 16) = make_uint4(0, 0, 0, 0);
-  __syncwarp();
+  if (lane == 0)
+    for (int s = 0; s < C::kStages; ++s) mbar_init(bar(s), 1);
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    prefetch_tensormap(&tk);
+    prefetch_tensormap(&tv);
+  }
+  fence_mbar_init();
+  fence_proxy_async_smem();
+  __syncthreads();
   grid_wait_previous();
   grid_allow_next();
 
@@ -193,147 +210,171 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   find_unit(a, heads, u0, lane, load);
   Walk work = load;
 
-  // ---- loading: unit n of the stretch into stage n % kStages; lane i looks after key i % 16 of the warp's 16
-  auto issue = [&](int stage) {
-    const int key = load.unit * kUnit + warp * 16 + (lane & 15);
-    int page = -1, slot = 0;
-    if (key < load.length) {
+  // ---- loading: unit n of the stretch into stage n % kStages; lane i looks after box i of the warp's 16 keys.  The page
+  // number of the next unit's box is on its way while this one is waited for and worked on.
+  const int boxes = 16 / box_rows;
+  int page = -1, slot = 0;
+  auto look_up = [&]() {
+    const int key = load.unit * kUnit + warp * 16 + lane * box_rows;
+    page = -1;
+    if (lane < boxes && key < load.length) {
       const int index = key / a.page_size;
       slot = key - index * a.page_size;
       page = ld_global(a.block_table + load.b * a.table_stride + index);
-      if (page < 0 || page >= a.pages) {
-        atomicCAS(status, 0, kStatusPage | kSiteDecode);
-        page = -1;
-      }
     }
-    const uint32_t here = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-    if (here != 0) {
-      const int kv_head = load.h / blocks;
-      const uint16_t* const kbase = static_cast<const uint16_t*>(a.k_cache) + kv_head * a.sk_cache.head;
-      const uint16_t* const vbase = static_cast<const uint16_t*>(a.v_cache) + kv_head * a.sv_cache.head;
+  };
+  int issued = 0;
+  auto issue = [&](int stage) {
+    const int key = load.unit * kUnit + warp * 16 + lane * box_rows;
+    const bool asked = lane < boxes && key < load.length;
+    const bool take = asked && page >= 0 && page < a.pages;
+    if (asked && !take) atomicCAS(status, 0, kStatusPage | kSiteDecode);
+    const int copies = __popc(__ballot_sync(0xffffffffu, take));
+    // keys of this lane's box that count
+    const int here = take ? min(load.length - key, box_rows) : 0;
+    uint32_t keys = here > 0 ? ((1u << here) - 1u) << (lane * box_rows) : 0u;
+    keys = __reduce_or_sync(0xffffffffu, keys);
+    if (copies != 0) {
       const uint32_t dst = ring + stage * 2 * C::kTileBytes;
+      if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * DP * 4);
+      __syncwarp();
+      if (take) {
+        const int kv_head = load.h / blocks;
 #pragma unroll
-      for (int i = 0; i < 16 * kPieces / 32; ++i) {
-        const int row = (lane + 32 * i) / kPieces, piece = (lane + 32 * i) % kPieces;
-        const int p = __shfl_sync(0xffffffffu, page, row), s = __shfl_sync(0xffffffffu, slot, row);
-        if (piece < d8) {
-          const uint32_t to = dst + row * (DP * 2) + ((piece ^ (row & 7)) << 4);
-          const bool take = p >= 0;  // zeros otherwise: their weight is zero, and 0 x NaN is none
-          const long long pp = take ? p : 0, sl = take ? s : 0;
-          copy16(to, kbase + pp * a.sk_cache.page + sl * a.sk_cache.slot + piece * 8, take);
-          copy16(to + C::kTileBytes, vbase + pp * a.sv_cache.page + sl * a.sv_cache.slot + piece * 8, take);
+        for (int ch = 0; ch < C::kChunks; ++ch) {
+          const uint32_t to = dst + ch * 2048 + lane * box_rows * 128;
+          tma_load_4d(to, &tk, ch * 64, slot, HeadCoord{kv_head, page}, bar(stage));
+          tma_load_4d(to + C::kTileBytes, &tv, ch * 64, slot, HeadCoord{kv_head, page}, bar(stage));
         }
       }
     }
-    return here;
-  };
-  uint32_t valid[C::kStages];  // which of its 16 keys the stage of unit n, n + 1, .. holds
-  int issued = 0;
-#pragma unroll
-  for (int s = 0; s < C::kStages; ++s) {
-    valid[s] = 0;
-    if (issued < count) {
-      valid[s] = issue(s);
-      if (++issued < count) next_unit(a, heads, load);
+    if (++issued < count) {
+      next_unit(a, heads, load);
+      look_up();
     }
-    copies_commit();
-  }
-
-  uint32_t qa[DP / 16][4];
-  float o[DP / 8][4];
-  float m[2], l[2];
-  bool fresh = true;
-  for (int n = 0; n < count; ++n) {
-    const int head0 = work.h / blocks * group + work.h % blocks * kRows;    // first query head of the rows
-    const int here = min(kRows, group - work.h % blocks * kRows);           // rows in use
-    if (fresh) {
-      fresh = false;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+    return keys;
+  };
+  look_up();
+  uint32_t valid[C::kStages];  // which of its 16 keys the stage of unit n, n + 1, .. holds
 #pragma unroll
-      for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int s = 0; s < C::kStages; ++s) valid[s] = issued < count ? issue(s) : 0u;
+
+  uint32_t qb[DP / 16][NT][2];
+  float o[DP / 16][NT][4];  // rows (columns of V) 16 i + lane / 4 (+ 8), columns (query heads) 8 t + 2 (lane % 4) (+ 1)
+  float m[NT][2], l[NT][2];
+  const float threshold = 8.f / a.scale_log2;
+  uint32_t phases = 0;  // bit s: parity of the next wait on stage s
+  bool fresh = true, ok = true;
+  int stage = 0;
+  for (int n = 0; n < count; ++n) {
+    const int head0 = work.h / blocks * group + work.h % blocks * kRows;  // first query head
+    const int here = min(kRows, group - work.h % blocks * kRows);         // query heads in use
+    if (fresh) {
       const uint16_t* const q = static_cast<const uint16_t*>(a.q) + work.b * a.sq.row;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
+      for (int t = 0; t < NT; ++t) {
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = lane / 4 + (i & 1) * 8, col = k * 16 + (lane & 3) * 2 + (i >> 1) * 8;
-          qa[k][i] = row < here && col < a.D
-                         ? ld_global(reinterpret_cast<const unsigned*>(q + (head0 + row) * a.sq.head + col)) : 0u;
+        for (int i = 0; i < DP / 16; ++i) {
+          o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int head = 8 * t + lane / 4, col = 16 * i + 8 * j + (lane & 3) * 2;
+            qb[i][t][j] = head < here && col < a.D
+                              ? ld_global(reinterpret_cast<const unsigned*>(q + (head0 + head) * a.sq.head + col)) : 0u;
+          }
         }
+      }
     }
     // ---- one unit: this warp's 16 keys
-    copies_wait<C::kStages - 1>();
-    __syncwarp();
     const uint32_t mine = valid[0];
     if (mine != 0) {
-      const uint32_t ktile = ring + (n % C::kStages) * 2 * C::kTileBytes, vtile = ktile + C::kTileBytes;
-      const int mrow = (lane & 7) + ((lane >> 4) << 3), mpiece = (lane >> 3) & 1;  // of this lane's matrix row
-      float s[2][4] = {};
+      if (ok) ok = mbar_wait_warp(bar(stage), (phases >> stage) & 1u, w, kSiteDecode);
+      phases ^= 1u << stage;
+      const uint32_t ktile = ring + stage * 2 * C::kTileBytes, vtile = ktile + C::kTileBytes;
+      if (mine != 0xffffu) {  // rows that do not count: 0 x NaN is none
+        for (int i = lane; i < 16 * C::kChunks * 8; i += 32)
+          if (!((mine >> (i / 8 % 16)) & 1u))
+            *reinterpret_cast<uint4*>(smem + (vtile - base) + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      // row of this lane in the 16 x 16 piece of a tile that ldmatrix takes, and which half of its columns
+      const int krow = (lane & 7) + (lane & 8), khalf = lane >> 4;
+      float s[NT][4] = {};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        uint32_t b[4];
-        load_matrices(ktile + mrow * (DP * 2) + (((2 * k + mpiece) ^ (mrow & 7)) << 4), b);
-        product<BF16>(s[0], qa[k], b[0], b[1]);
-        product<BF16>(s[1], qa[k], b[2], b[3]);
+        uint32_t x[4];
+        load_matrices(ktile + (k / 4) * 2048 + krow * 128 + (((2 * (k % 4) + khalf) ^ (krow & 7)) << 4), x);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) product<BF16>(s[t], x, qb[k][t][0], qb[k][t][1]);
       }
-      if (mine != 0xffffu) {
+      const bool in0 = (mine >> (lane / 4)) & 1u, in1 = (mine >> (lane / 4 + 8)) & 1u;
+      bool need = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!((mine >> (t * 8 + (lane & 3) * 2 + (i & 1))) & 1u)) s[t][i] = -INFINITY;
-      }
-      float alpha[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        const float was = m[r];
-        m[r] = fmaxf(was, x);
-        // a row without a finite score so far has weights 0
-        alpha[r] = m[r] == -INFINITY ? 1.f : ex2((was - m[r]) * a.scale_log2);
-        const float base = m[r] == -INFINITY ? 0.f : -m[r] * a.scale_log2;
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) sum += s[t][2 * r + e] = ex2(fmaf(s[t][2 * r + e], a.scale_log2, base));
-        l[r] = l[r] * alpha[r] + sum;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          o[i][0] *= alpha[0], o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1], o[i][3] *= alpha[1];
+        for (int e = 0; e < 2; ++e) {
+          if (!in0) s[t][e] = -INFINITY;
+          if (!in1) s[t][2 + e] = -INFINITY;
+          need |= fmaxf(s[t][e], s[t][2 + e]) - m[t][e] > threshold;
         }
+      // The maximum follows only when a score is 2^8 above it: a weight is at most 2^8 then.
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[t][e], s[t][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x = fmaxf(x, m[t][e]);
+            // a head without a finite score so far has weights 0
+            const float alpha = x == -INFINITY ? 1.f : ex2((m[t][e] - x) * a.scale_log2);
+            m[t][e] = x;
+            l[t][e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) o[i][t][e] *= alpha, o[i][t][2 + e] *= alpha;
+          }
       }
-      // P in 16 bits; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
+      // P^T in 16 bits; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
       // term is p (1 - 2^-8) rounded, at most p (1 - 2^-16), so that the second one is positive where p is, and an
       // infinite value stays infinite in both products.
-      uint32_t p[4], rest[4];
+      uint32_t p[NT][2], rest[NT][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = s[i >> 1][2 * (i & 1)], y = s[i >> 1][2 * (i & 1) + 1];
-        if constexpr (BF16) {
-          p[i] = pack2<BF16>(x * 0.99609375f, y * 0.99609375f);
-          const float2 f = unpack2<BF16>(p[i]);
-          rest[i] = pack2<BF16>(x - f.x, y - f.y);
-        } else {
-          p[i] = pack2<BF16>(x, y);
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float shift = m[t][e] == -INFINITY ? 0.f : -m[t][e] * a.scale_log2;
+          s[t][e] = ex2(fmaf(s[t][e], a.scale_log2, shift));
+          s[t][2 + e] = ex2(fmaf(s[t][2 + e], a.scale_log2, shift));
+          l[t][e] += s[t][e] + s[t][2 + e];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x = s[t][2 * j], y = s[t][2 * j + 1];
+          if constexpr (BF16) {
+            const uint32_t both = pack2<BF16>(x * 0.99609375f, y * 0.99609375f);
+            const float2 f = unpack2<BF16>(both);
+            p[t][j] = turned(both);
+            rest[t][j] = turned(pack2<BF16>(x - f.x, y - f.y));
+          } else {
+            p[t][j] = turned(pack2<BF16>(x, y));
+          }
         }
       }
+      // V^T: the 16 x 16 piece of V is turned around on its way, so the lanes' rows and halves change places
+      const int vrow = (lane & 7) + ((lane >> 4) << 3), vhalf = (lane >> 3) & 1;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        uint32_t b[4];
-        const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vpiece = lane >> 4;
-        load_matrices_t(vtile + vrow * (DP * 2) + (((2 * k + vpiece) ^ (vrow & 7)) << 4), b);
-        product<BF16>(o[2 * k], p, b[0], b[1]);
-        product<BF16>(o[2 * k + 1], p, b[2], b[3]);
-        if constexpr (BF16) {
-          product<BF16>(o[2 * k], rest, b[0], b[1]);
-          product<BF16>(o[2 * k + 1], rest, b[2], b[3]);
+      for (int i = 0; i < DP / 16; ++i) {
+        uint32_t x[4];
+        load_matrices_t(vtile + (i / 4) * 2048 + vrow * 128 + (((2 * (i % 4) + vhalf) ^ (vrow & 7)) << 4), x);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          product<BF16>(o[i][t], x, p[t][0], p[t][1]);
+          if constexpr (BF16) product<BF16>(o[i][t], x, rest[t][0], rest[t][1]);
         }
       }
     }
@@ -341,16 +382,13 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     // ---- the next load takes the stage of this unit
 #pragma unroll
     for (int s = 0; s + 1 < C::kStages; ++s) valid[s] = valid[s + 1];
-    valid[C::kStages - 1] = 0;
-    if (issued < count) {
-      valid[C::kStages - 1] = issue(n % C::kStages);
-      if (++issued < count) next_unit(a, heads, load);
-    }
-    copies_commit();
+    valid[C::kStages - 1] = ok && issued < count ? issue(stage) : 0u;
+    if (++stage == C::kStages) stage = 0;
 
-    // ---- the end of a (sequence, key head), or of the stretch: the warps' sums become one, eight rows at a time
+    // ---- the end of a (sequence, key head), or of the stretch: the warps' sums become one, eight heads at a time
     const bool ends = work.unit + 1 == work.units;
-    if (ends || n + 1 == count) {
+    fresh = ends || n + 1 == count;
+    if (fresh) {
       const bool begins = work.unit <= n;  // its first unit is in this stretch
       const bool whole = begins && ends;
       float* const part = partial(a.workspace, gridDim.x, 2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
@@ -361,33 +399,34 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
         *reinterpret_cast<int4*>(cut) = make_int4(work.b, work.h, cta, count);
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (r * kJoinRows >= here) break;
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        {
-          const int row = lane / 4;
-          float* const to = join + (warp * kJoinRows + row) * C::kJoinStride;
+      for (int t = 0; t < NT; ++t) {
+        const int row0 = t * kJoinRows, some = min(here - row0, kJoinRows);
+        if (some <= 0) break;
 #pragma unroll
-          for (int i = 0; i < DP / 8; ++i)
-            *reinterpret_cast<float2*>(to + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
-          if ((lane & 3) == 0)
-            *reinterpret_cast<float2*>(join_ml + (warp * kJoinRows + row) * 2) = make_float2(m[r], l[r]);
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[t][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int row = warp * kJoinRows + (lane & 3) * 2 + e;
+          float* const to = join + row * C::kJoinStride + lane / 4;
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) to[16 * i] = o[i][t][e], to[16 * i + 8] = o[i][t][2 + e];
+          if (lane < 4) *reinterpret_cast<float2*>(join_ml + row * 2) = make_float2(m[t][e], sum);
         }
         __syncthreads();
-        const int row0 = r * kJoinRows, some = min(here - row0, kJoinRows);
         for (int i = threadIdx.x; i < some * (a.D / 2); i += 32 * kWarps) {
           const int row = i / (a.D / 2), col = (i - row * (a.D / 2)) * 2;
           float mw[kWarps], top = -INFINITY;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mw[w] = join_ml[(w * kJoinRows + row) * 2]);
+          for (int v = 0; v < kWarps; ++v) top = fmaxf(top, mw[v] = join_ml[(v * kJoinRows + row) * 2]);
           float2 sum = make_float2(0.f, 0.f);
           float all = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float lw = join_ml[(w * kJoinRows + row) * 2 + 1];
-            const float f = part_weight(mw[w], lw, top, a.scale_log2);
-            const float2 x = *reinterpret_cast<const float2*>(join + (w * kJoinRows + row) * C::kJoinStride + col);
+          for (int v = 0; v < kWarps; ++v) {
+            const float lw = join_ml[(v * kJoinRows + row) * 2 + 1];
+            const float f = part_weight(mw[v], lw, top, a.scale_log2);
+            const float2 x = *reinterpret_cast<const float2*>(join + (v * kJoinRows + row) * C::kJoinStride + col);
             sum.x = fmaf(f, x.x, sum.x);
             sum.y = fmaf(f, x.y, sum.y);
             all = fmaf(f, lw, all);
@@ -403,7 +442,6 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
         }
         __syncthreads();
       }
-      fresh = true;
     }
     if (n + 1 < count) next_unit(a, heads, work);
   }
@@ -415,7 +453,8 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
 // 73 us on two sequences of 131072 keys.
 constexpr int kJoinThreads = 256;
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass,
+                                                                   int ctas) {
   __shared__ float weight[kJoinThreads], reduced[kJoinThreads / 32];
   __shared__ float2 sums[kJoinThreads];
   grid_wait_previous();
@@ -423,8 +462,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
   const int c0 = blockIdx.x / rows, row = blockIdx.x - c0 * rows;
   const uint4* const cuts = reinterpret_cast<const uint4*>(a.workspace);
   const uint4 cut = ld_global(cuts + c0);  // a Cut
-  const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
-  const int h = static_cast<int>(cut.y), kv_head = h / blocks, in_group = (h - kv_head * blocks) * kRows + row;
+  const int group = a.Hq / a.Hkv, blocks = (group + pass - 1) / pass;  // pass: query heads that one pass takes
+  const int h = static_cast<int>(cut.y), kv_head = h / blocks, in_group = (h - kv_head * blocks) * pass + row;
   if (static_cast<int>(cut.z) < 0 || in_group >= group) return;
   const int parts = static_cast<int>(cut.z) - c0 + 1, d2 = a.D / 2;
   const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = kJoinThreads / d2;
@@ -485,44 +524,55 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
   }
 }
 
-// CTAs of decode_kernel.
-int decode_ctas(const DecodeArgs& a, int per_sm, int num_sms) {
-  const int blocks = (a.Hq / a.Hkv + kRows - 1) / kRows;
-  const long long units = (static_cast<long long>(a.table_width) * a.page_size + kUnit - 1) / kUnit;
-  const long long most = units * a.batch * a.Hkv * blocks;
-  const long long slots = static_cast<long long>(num_sms) * per_sm;
-  return static_cast<int>(most < slots ? most : (slots < kMaxCtas ? slots : kMaxCtas));
+// Units of the call at most, and CTAs of decode_kernel.
+long long most_units(int batch, int Hq, int Hkv, int table_width, int page_size) {
+  const int group = Hq / Hkv, pass = 8 * column_tiles(group);
+  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit;
+  return units * batch * Hkv * ((group + pass - 1) / pass);
 }
 
-template <int DP, bool BF16>
-cudaError_t launch_decode_t(const DecodeArgs& a, int num_sms, int* status, cudaStream_t stream) {
+template <int DP, int NT, bool BF16>
+cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int box_rows, int num_sms, int* status,
+                            cudaStream_t stream) {
   using C = DecodeCfg<DP>;
-  auto kern = decode_kernel<DP, BF16>;
-  const int group = a.Hq / a.Hkv, rows = group < kRows ? group : kRows;
+  auto kern = decode_kernel<DP, NT, BF16>;
+  const int group = a.Hq / a.Hkv, rows = group < 8 * NT ? group : 8 * NT;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  const int ctas = decode_ctas(a, C::kCtasPerSm, num_sms);
-  e = launch_dependent(kern, ctas, 32 * kWarps, C::kSmemBytes, stream, a, rows, status);
+  const long long most = most_units(a.batch, a.Hq, a.Hkv, a.table_width, a.page_size), slots = static_cast<long long>(num_sms) * C::kCtasPerSm;
+  const int ctas = static_cast<int>(most < slots ? most : (slots < kMaxCtas ? slots : kMaxCtas));
+  e = launch_dependent(kern, ctas, 32 * kWarps, C::kSmemBytes, stream, tk, tv, a, rows, box_rows, status);
   if (e != cudaSuccess) return e;
-  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(ctas) * rows, kJoinThreads, 0, stream, a, rows, ctas);
+  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(ctas) * rows, kJoinThreads, 0, stream, a, rows, 8 * NT, ctas);
 }
 
 }  // namespace
 
 size_t decode_workspace_floats(int batch, int Hq, int Hkv, int D, int table_width, int page_size) {
-  const int group = Hq / Hkv, blocks = (group + kRows - 1) / kRows, rows = group < kRows ? group : kRows;
-  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit;
-  const long long most = units * batch * Hkv * blocks;
-  const long long ctas = most < kMaxCtas ? most : kMaxCtas;
+  const int group = Hq / Hkv, pass = 8 * column_tiles(group), rows = group < pass ? group : pass;
+  const long long most = most_units(batch, Hq, Hkv, table_width, page_size), ctas = most < kMaxCtas ? most : kMaxCtas;
   return static_cast<size_t>(ctas) * (4 + 2 * rows * (D + 2));
 }
 
-cudaError_t launch_decode(const DecodeArgs& a, int dtype, int num_sms, int* status, cudaStream_t stream) {
-  if (a.D <= 64)
-    return dtype ? launch_decode_t<64, true>(a, num_sms, status, stream) : launch_decode_t<64, false>(a, num_sms, status, stream);
-  if (a.D <= 128)
-    return dtype ? launch_decode_t<128, true>(a, num_sms, status, stream) : launch_decode_t<128, false>(a, num_sms, status, stream);
-  return dtype ? launch_decode_t<256, true>(a, num_sms, status, stream) : launch_decode_t<256, false>(a, num_sms, status, stream);
+int decode_box_rows(int page_size) {
+  int rows = 16;
+  while (page_size % rows) rows /= 2;
+  return rows;
+}
+
+cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int dtype, int num_sms, int* status,
+                          cudaStream_t stream) {
+  const int box = decode_box_rows(a.page_size), tiles = column_tiles(a.Hq / a.Hkv);
+#define FA2_CASE(DP)                                                                                         \
+  if (tiles == 1)                                                                                            \
+    return dtype ? launch_decode_t<DP, 1, true>(tk, tv, a, box, num_sms, status, stream)                     \
+                 : launch_decode_t<DP, 1, false>(tk, tv, a, box, num_sms, status, stream);                   \
+  return dtype ? launch_decode_t<DP, 2, true>(tk, tv, a, box, num_sms, status, stream)                       \
+               : launch_decode_t<DP, 2, false>(tk, tv, a, box, num_sms, status, stream)
+  if (a.D <= 64) { FA2_CASE(64); }
+  if (a.D <= 128) { FA2_CASE(128); }
+  FA2_CASE(256);
+#undef FA2_CASE
 }
 
 }  // namespace fa2

@@ -1,6 +1,7 @@
 // Arguments of the kernels that work on a paged key-value cache: tensors [pages, page_size, Hkv, D] whose pages a
 // block table [batch, table_width] hands out to the sequences.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace fa2 {
@@ -47,6 +48,10 @@ struct DecodeArgs {
   float scale_log2;
 };
 size_t decode_workspace_floats(int batch, int Hq, int Hkv, int D, int table_width, int page_size);
-cudaError_t launch_decode(const DecodeArgs& a, int dtype, int num_sms, int* status, cudaStream_t stream);
+// Rows of the boxes that the cache's tensor maps bring in: the largest part of 16 that divides a page.
+int decode_box_rows(int page_size);
+// tk, tv: maps (D, slots, heads, pages) with boxes (64, decode_box_rows, 1, 1), 128-byte swizzle.
+cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int dtype, int num_sms, int* status,
+                          cudaStream_t stream);
 
 }  // namespace fa2
