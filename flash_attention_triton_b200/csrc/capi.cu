@@ -119,7 +119,7 @@ int get_strides(const long long* user, int idx, int B, int H, int N, int D, Stri
 }  // namespace
 
 int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D, const Strides& st,
-               int box_columns, int box_rows, CUtensorMapSwizzle swizzle) {
+               int box_columns, int box_rows, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return FA2_ERR_DRIVER;
   const cuuint64_t gdim[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(N),
@@ -132,7 +132,7 @@ int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N,
   const CUresult r =
       enc(m, dtype ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
           const_cast<void*>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+          promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? FA2_OK : FA2_ERR_DRIVER;
 }
 

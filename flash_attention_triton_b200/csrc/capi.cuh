@@ -12,7 +12,8 @@ int launch_context(LaunchCtx* ctx);
 
 // Tensor map over a [B, H, N, D] 16-bit tensor with box (box_columns, box_rows, 1, 1).
 int encode_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int N, int D, const Strides& st,
-               int box_columns, int box_rows, CUtensorMapSwizzle swizzle);
+               int box_columns, int box_rows, CUtensorMapSwizzle swizzle,
+               CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 // The same with box (chunk, box_rows, 1, 1).  The chunk
 // follows the padded head dim, so for D = 48 or 96 the last box of a row hangs over the
 // tensor: those columns read as zeros and are not written.

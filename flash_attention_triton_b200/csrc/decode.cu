@@ -6,7 +6,8 @@
 // units of the call stand in one row, and each CTA takes an equal stretch of it, whatever the lengths are, so
 // one long sequence and many short ones both keep every SM reading.  Where a stretch cuts a (sequence, key head)
 // apart, each CTA leaves (m, l, o) of its part in the workspace, and decode_join_kernel adds the parts up in order:
-// the same bits every time.
+// the same bits every time.  Where a key head has more query heads than one pass takes, neighbouring CTAs take the same
+// stretch with 16 of them each, at the same time, so that the L2 serves all but the first.
 //
 // Inside a CTA warp w takes keys 16 w .. 16 w + 15 of every unit and runs on its own: tiled copies bring its keys and
 // values into a ring of stages of its own, as many rows to a copy as 16 keys have next to each other in a page (16 where
@@ -15,6 +16,8 @@
 // movmatrix.  Eight query heads fill the product; as its rows they would fill half of it.  The four warps meet
 // where a (sequence, key head) ends, while their next stages are already loading.  The products take a fraction of
 // the time that the bytes take, so mma.sync serves, and a row of eight queries needs no tile of 128.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
@@ -44,9 +47,9 @@ struct DecodeCfg {
   static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of one SM");
 };
 
-// One (sequence, row of heads) of the call, and the walk over the units of a CTA's stretch.
+// One (sequence, key head) of the call, and the walk over the units of a CTA's stretch.
 struct Walk {
-  int b, h;        // sequence; key head and, where it has more than 16 query heads, which 16 of them
+  int b, h;
   int unit;        // next unit of it
   int units;       // units of the sequence
   int length;      // keys of the sequence
@@ -144,22 +147,30 @@ __device__ __forceinline__ float part_weight(float m, float l, float top, float 
   return m == -INFINITY ? l * 0.f : ex2((m - top) * scale_log2);
 }
 
-// The workspace: for each CTA what it has begun and not ended, then the partial results.  CTA c has two places for those,
-// 2 c for the part that continues what the CTA before began and 2 c + 1 for the one that it begins; a place is m, l of
-// `rows` rows and their o.
+// The workspace: who has cut what, how many units each CTA had, then the partial results.  A Cut belongs to a (sequence,
+// key head, pass) where the call has fewer of those than CTAs, else to the CTA that begins it, so that decode_join_kernel
+// looks at few of them.  CTA c has two places for partial results, 2 c for the part that continues what the CTA before began
+// and 2 c + 1 for the one that it begins; a place is m, l of `rows` rows and their o.
 struct Cut {
-  int b, h;  // as in Walk
-  int last;  // CTA that has the last unit; below 0: it has ended what it began
-  int units; // of the CTA's stretch
+  int b, h;         // as in Walk
+  int first, last;  // stretches that have its first and its last unit; last below 0: it is not cut
 };
-__device__ __forceinline__ float* partial(float* workspace, int ctas, int place, int rows, int D) {
-  return workspace + ctas * 4 + static_cast<long long>(place) * rows * (D + 2);
-}
+struct Workspace {
+  int4* cuts;
+  int* counts;
+  float* parts;
+  __host__ __device__ static long long floats(long long slots, long long ctas, int rows, int D) {
+    return 4 * slots + (ctas + 3) / 4 * 4 + 2 * ctas * rows * (D + 2);
+  }
+  __device__ Workspace(float* p, int slots, int ctas)
+      : cuts(reinterpret_cast<int4*>(p)), counts(reinterpret_cast<int*>(p + 4 * slots)), parts(p + 4 * slots + (ctas + 3) / 4 * 4) {}
+  __device__ float* part(int place, int rows, int D) const { return parts + static_cast<long long>(place) * rows * (D + 2); }
+};
 
 template <int DP, int NT, bool BF16>
 __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                  const __grid_constant__ DecodeArgs a, int rows, int box_rows, int* status) {
+                  const __grid_constant__ DecodeArgs a, int rows, int slots, int box_rows, int* status) {
   using C = DecodeCfg<DP>;
   constexpr int kRows = 8 * NT;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -176,7 +187,8 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffAbort);
   const WaitCtx w{abort_flag, status};
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
-  const int heads = a.Hkv * blocks;
+  const int stretches = gridDim.x / blocks, stretch = blockIdx.x / blocks, pass = blockIdx.x - stretch * blocks;
+  const int heads = a.Hkv;
   const int d8 = a.D / 8;
 
   if (lane == 0)
@@ -192,18 +204,23 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   grid_wait_previous();
   grid_allow_next();
 
+  const Workspace space(a.workspace, slots, gridDim.x);
+  const bool by_segment = static_cast<long long>(a.batch) * heads * blocks == slots;  // what a Cut belongs to
   // sequences without keys
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (ld_global(a.lengths + b) <= 0)
+    if (ld_global(a.lengths + b) <= 0) {
       for (int i = threadIdx.x; i < a.Hq * d8; i += 32 * kWarps)
         reinterpret_cast<uint4*>(a.out)[static_cast<long long>(b) * a.Hq * d8 + i] = make_uint4(0, 0, 0, 0);
+      if (by_segment)
+        for (int h = threadIdx.x; h < heads * blocks; h += 32 * kWarps) space.cuts[b * heads * blocks + h] = make_int4(0, 0, 0, -1);
+    }
 
   const long long total = units_before(a, a.batch, lane) * heads;
-  const long long u0 = stretch_start(total, blockIdx.x, gridDim.x);
-  const int count = static_cast<int>(stretch_start(total, blockIdx.x + 1, gridDim.x) - u0);
-  Cut* const cut = reinterpret_cast<Cut*>(a.workspace) + blockIdx.x;
+  const long long u0 = stretch_start(total, stretch, stretches);
+  const int count = static_cast<int>(stretch_start(total, stretch + 1, stretches) - u0);
+  if (threadIdx.x == 0) space.counts[blockIdx.x] = count;
   if (count == 0) {
-    if (threadIdx.x == 0) *reinterpret_cast<int4*>(cut) = make_int4(0, 0, -1, 0);
+    if (!by_segment && threadIdx.x == 0) space.cuts[blockIdx.x] = make_int4(0, 0, 0, -1);
     return;
   }
   Walk load;
@@ -239,7 +256,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
       if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * DP * 4);
       __syncwarp();
       if (take) {
-        const int kv_head = load.h / blocks;
+        const int kv_head = load.h;
 #pragma unroll
         for (int ch = 0; ch < C::kChunks; ++ch) {
           const uint32_t to = dst + ch * 2048 + lane * box_rows * 128;
@@ -266,9 +283,9 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   uint32_t phases = 0;  // bit s: parity of the next wait on stage s
   bool fresh = true, ok = true;
   int stage = 0;
+  const int here = min(kRows, group - pass * kRows);  // query heads in use
   for (int n = 0; n < count; ++n) {
-    const int head0 = work.h / blocks * group + work.h % blocks * kRows;  // first query head
-    const int here = min(kRows, group - work.h % blocks * kRows);         // query heads in use
+    const int head0 = work.h * group + pass * kRows;  // the first one
     if (fresh) {
       const uint16_t* const q = static_cast<const uint16_t*>(a.q) + work.b * a.sq.row;
 #pragma unroll
@@ -391,12 +408,12 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     if (fresh) {
       const bool begins = work.unit <= n;  // its first unit is in this stretch
       const bool whole = begins && ends;
-      float* const part = partial(a.workspace, gridDim.x, 2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
-      if (n + 1 == count && threadIdx.x == 0) {
-        // the CTA of a unit is the last one whose stretch starts at or before it
+      float* const part = space.part(2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
+      if (threadIdx.x == 0 && (by_segment ? begins : n + 1 == count)) {
+        // the stretch of a unit is the last one that starts at or before it
         const long long last = u0 + n + (work.units - 1 - work.unit);
-        const int cta = begins && !ends ? static_cast<int>(((last + 1) * gridDim.x - 1) / total) : -1;
-        *reinterpret_cast<int4*>(cut) = make_int4(work.b, work.h, cta, count);
+        const int end = begins && !ends ? static_cast<int>(((last + 1) * stretches - 1) / total) : -1;
+        space.cuts[by_segment ? (work.b * heads + work.h) * blocks + pass : blockIdx.x] = make_int4(work.b, work.h, stretch, end);
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -447,27 +464,28 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   }
 }
 
-// Adds up the parts of what decode_kernel's stretches cut apart: block (c, row) one query head of what CTA c began and did
-// not end.  First the weights of all parts, one a thread, then the parts, D / 2 threads to each, so that no load waits for
+// Adds up the parts of what decode_kernel's stretches cut apart: block (c, row) one query head of Cut c.  First the weights of all parts, one a thread, then the parts, D / 2 threads to each, so that no load waits for
 // another.  Few long sequences have a hundred parts and more to a head: one thread a column, part after part, took
 // 73 us on two sequences of 131072 keys.
 constexpr int kJoinThreads = 256;
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass,
-                                                                   int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass_heads,
+                                                                   int slots, int ctas) {
   __shared__ float weight[kJoinThreads], reduced[kJoinThreads / 32];
   __shared__ float2 sums[kJoinThreads];
   grid_wait_previous();
   grid_allow_next();
-  const int c0 = blockIdx.x / rows, row = blockIdx.x - c0 * rows;
-  const uint4* const cuts = reinterpret_cast<const uint4*>(a.workspace);
-  const uint4 cut = ld_global(cuts + c0);  // a Cut
-  const int group = a.Hq / a.Hkv, blocks = (group + pass - 1) / pass;  // pass: query heads that one pass takes
-  const int h = static_cast<int>(cut.y), kv_head = h / blocks, in_group = (h - kv_head * blocks) * pass + row;
-  if (static_cast<int>(cut.z) < 0 || in_group >= group) return;
-  const int parts = static_cast<int>(cut.z) - c0 + 1, d2 = a.D / 2;
+  const Workspace space(a.workspace, slots, ctas);
+  const uint4 c = ld_global(reinterpret_cast<const uint4*>(space.cuts) + blockIdx.x / rows);
+  const Cut cut{static_cast<int>(c.x), static_cast<int>(c.y), static_cast<int>(c.z), static_cast<int>(c.w)};
+  const int row = blockIdx.x % rows;
+  const int group = a.Hq / a.Hkv, blocks = (group + pass_heads - 1) / pass_heads, pass = blockIdx.x / rows % blocks;
+  const int in_group = pass * pass_heads + row;
+  if (cut.last < 0 || in_group >= group) return;
+  const int parts = cut.last - cut.first + 1, d2 = a.D / 2;
   const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = kJoinThreads / d2;
-  auto part = [&](int i) { return partial(a.workspace, ctas, 2 * (c0 + i) + (i == 0 ? 1 : 0), rows, a.D); };
+  auto cta = [&](int i) { return (cut.first + i) * blocks + pass; };
+  auto part = [&](int i) { return space.part(2 * cta(i) + (i == 0 ? 1 : 0), rows, a.D); };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top = -INFINITY, all = 0.f;
   float2 sum = make_float2(0.f, 0.f);
@@ -475,7 +493,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
     const int here = min(parts - p0, kJoinThreads);
     float m = -INFINITY, l = 0.f;
     // a CTA without units (there are fewer units than CTAs) has left nothing
-    if (threadIdx.x < here && ld_global(cuts + c0 + p0 + threadIdx.x).w != 0) {
+    if (threadIdx.x < here && ld_global(space.counts + cta(p0 + threadIdx.x)) != 0) {
       const float* const at = part(p0 + threadIdx.x) + 2 * row;
       m = ld_global(at), l = ld_global(at + 1);
     }
@@ -501,13 +519,13 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
 #pragma unroll
     for (int i = 0; i < kJoinThreads / 32; ++i) all += reduced[i];
     if (share < shares)
-#pragma unroll 4
+#pragma unroll 8
       for (int i = share; i < here; i += shares) {
         const float f = weight[i];
-        if (f == 0.f) continue;
-        const float* const x = part(p0 + i) + 2 * rows + row * a.D + 2 * col;
-        sum.x = fmaf(f, ld_global(x), sum.x);
-        sum.y = fmaf(f, ld_global(x + 1), sum.y);
+        const float2 x = ld_global(reinterpret_cast<const float2*>(part(p0 + i) + 2 * rows + row * a.D + 2 * col));
+        // (weight 0: the part may have been left out, and hold anything)
+        sum.x = f == 0.f ? sum.x : fmaf(f, x.x, sum.x);
+        sum.y = f == 0.f ? sum.y : fmaf(f, x.y, sum.y);
       }
     __syncthreads();
   }
@@ -519,16 +537,21 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
       sum.x += x.x, sum.y += x.y;
     }
     const float inv = 1.f / all;  // NaN for a row without any finite score, as everywhere
-    uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.x) * a.Hq + kv_head * group + in_group) * a.D + 2 * col;
+    uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.b) * a.Hq + cut.h * group + in_group) * a.D + 2 * col;
     *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(sum.x * inv, sum.y * inv);
   }
 }
 
-// Units of the call at most, and CTAs of decode_kernel.
-long long most_units(int batch, int Hq, int Hkv, int table_width, int page_size) {
-  const int group = Hq / Hkv, pass = 8 * column_tiles(group);
-  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit;
-  return units * batch * Hkv * ((group + pass - 1) / pass);
+// CTAs of decode_kernel, of `slots` that run at a time: a multiple of the passes, no more than units of the call.
+struct DecodeGrid {
+  int rows, passes, ctas, cuts;
+};
+DecodeGrid decode_grid(int batch, int Hq, int Hkv, int table_width, int page_size, int slots) {
+  const int group = Hq / Hkv, take = 8 * column_tiles(group), passes = (group + take - 1) / take;
+  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit * batch * Hkv;
+  const long long stretches = std::max(1, slots / passes), segments = static_cast<long long>(batch) * Hkv * passes;
+  const int ctas = static_cast<int>(std::min(units, stretches) * passes);
+  return DecodeGrid{std::min(group, take), passes, ctas, static_cast<int>(std::min<long long>(segments, ctas))};
 }
 
 template <int DP, int NT, bool BF16>
@@ -536,22 +559,21 @@ cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const 
                             cudaStream_t stream) {
   using C = DecodeCfg<DP>;
   auto kern = decode_kernel<DP, NT, BF16>;
-  const int group = a.Hq / a.Hkv, rows = group < 8 * NT ? group : 8 * NT;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  const long long most = most_units(a.batch, a.Hq, a.Hkv, a.table_width, a.page_size), slots = static_cast<long long>(num_sms) * C::kCtasPerSm;
-  const int ctas = static_cast<int>(most < slots ? most : (slots < kMaxCtas ? slots : kMaxCtas));
-  e = launch_dependent(kern, ctas, 32 * kWarps, C::kSmemBytes, stream, tk, tv, a, rows, box_rows, status);
+  const DecodeGrid g = decode_grid(a.batch, a.Hq, a.Hkv, a.table_width, a.page_size, std::min(num_sms * C::kCtasPerSm, kMaxCtas));
+  e = launch_dependent(kern, g.ctas, 32 * kWarps, C::kSmemBytes, stream, tk, tv, a, g.rows, g.cuts, box_rows, status);
   if (e != cudaSuccess) return e;
-  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(ctas) * rows, kJoinThreads, 0, stream, a, rows, 8 * NT, ctas);
+  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows, kJoinThreads, 0, stream, a, g.rows, 8 * NT, g.cuts,
+                          g.ctas);
 }
 
 }  // namespace
 
 size_t decode_workspace_floats(int batch, int Hq, int Hkv, int D, int table_width, int page_size) {
-  const int group = Hq / Hkv, pass = 8 * column_tiles(group), rows = group < pass ? group : pass;
-  const long long most = most_units(batch, Hq, Hkv, table_width, page_size), ctas = most < kMaxCtas ? most : kMaxCtas;
-  return static_cast<size_t>(ctas) * (4 + 2 * rows * (D + 2));
+  // (more CTAs than this never run; the largest number of passes may need more)
+  const DecodeGrid g = decode_grid(batch, Hq, Hkv, table_width, page_size, kMaxCtas);
+  return static_cast<size_t>(Workspace::floats(g.cuts, g.ctas, g.rows, D));
 }
 
 int decode_box_rows(int page_size) {
