@@ -41,6 +41,17 @@ void check_code(const char* fn, int code) {
     throw error;
   }
 }
+
+void check_status_if_asked(const char* fn, const at::Tensor& on) {
+  const char* check = std::getenv("FA2_B200_CHECK_STATUS");
+  if (!check || std::strcmp(check, "1") != 0) return;
+  try {
+    pybind11::module_::import("flash_attention_triton_b200.api").attr("_check_status_if_asked")(fn, on.device());
+  } catch (pybind11::error_already_set& e) {
+    e.restore();
+    throw python_error();
+  }
+}
 }  // namespace fa2_host
 
 using fa2_host::check_code;

@@ -19,6 +19,9 @@ namespace fa2_host {
 // Raises _lib.Fa2Error for a non-zero code.  Called without the interpreter lock.
 void check_code(const char* fn, int code);
 
+// FA2_B200_CHECK_STATUS=1: raises _lib.Fa2Error when the status word of the device is set.  Called with the interpreter lock.
+void check_status_if_asked(const char* fn, const at::Tensor& on);
+
 inline int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FA2_DTYPE_FP16 : FA2_DTYPE_BF16; }
 inline bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 

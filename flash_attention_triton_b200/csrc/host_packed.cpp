@@ -121,6 +121,7 @@ PyObject* packed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const bool graph = c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
     result = graph ? PackedAttention::apply(q, k, v, in, cu, r, scale) : r.out;
   }
+  check_status_if_asked("fa2_packed_fwd", q);
   return THPVariable_Wrap(result);
   END_HANDLE_TH_ERRORS
 }

@@ -138,6 +138,7 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (const at::Tensor* t : {&k_cache, &v_cache})  // autograd sees that they have been written
       if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   }
+  check_status_if_asked("fa2_kv_append", k);
   return Py_BuildValue("NN", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
   END_HANDLE_TH_ERRORS
 }
@@ -173,6 +174,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                         c.page_size, c.table_width, dtype_code(q), static_cast<float>(scale), strides,
                                         c10::cuda::getCurrentCUDAStream(q.device().index()).stream()));
   }
+  check_status_if_asked("fa2_decode", q);
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }

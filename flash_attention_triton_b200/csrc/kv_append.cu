@@ -6,9 +6,15 @@
 //     (x1 cos - x2 sin, x2 cos + x1 sin),  in fp32, rounded once.
 //
 // Bound by memory for prompts (every element is read once and written once) and by latency for single tokens.
-// A thread has one place of a token's row for good: 16 bytes of one head, or the two 16-byte pieces that the
-// rotation joins; the token loop around it only adds strides.  A warp of the CTA finds sequence, position and
-// page of the CTA's tokens once (one binary search per token) and leaves them in shared memory.
+// A thread has one place of the heads' columns for good and takes four 16-byte pieces of one token at a time: the two pieces
+// that the rotation joins in two heads, or the same piece in four.  Their loads are in flight together, and the cosines and
+// sines are read once for all of them.  Many small CTAs: one loads while others look up places or store.  The first
+// warp of a CTA finds sequence, position and page of the CTA's tokens and leaves them in shared memory.
+// 31 323 tokens of 32 + 8 + 8 heads of 128 columns: 140 us, 91 % of the measured copy rate; with one head a thread, each token
+// behind the stores of the one before, 183 us, with 512 threads to a CTA 178 us, five and six CTAs of 256 threads on an SM
+// (48 and 40 registers, spilled) 148 and 161 us.
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.cuh"
 #include "ptx.cuh"
@@ -48,27 +54,65 @@ __device__ __forceinline__ void store16(void* base, long long element, const uin
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + element) = v;
 }
 
+// The sequence of a row: the first s with cu_seqlens[s + 1] > row, `batch` behind the last.  A warp looks at 32 places at once.
+__device__ __forceinline__ int sequence_of(const int* cu_seqlens, int batch, int row, int lane) {
+  int low = 0, high = batch;
+  while (low < high) {
+    const int step = (high - low + 31) / 32;
+    const int at = min(low + (lane + 1) * step, high);  // cu_seqlens[at] <= row: the answer is at least `at`
+    const int below = __popc(__ballot_sync(0xffffffffu, low + lane * step < high && ld_global(cu_seqlens + at) <= row));
+    high = min(low + (below + 1) * step, high) - 1;
+    low = min(low + below * step, high + 1);
+    if (step == 1) break;
+  }
+  return low;
+}
+
+// How threads share a token's row: first those with a pair of pieces in the heads of q and k (q's heads first), then those
+// with a single piece there, then those with a piece in the heads of v.  Of the threads that have the same place, j of
+// `groups` takes heads j, j + groups, ..
+constexpr int kPieces = 4;
+struct AppendShares {
+  int pairs, singles;  // places of a head of q or k
+  int pair_groups, single_groups, v_groups;
+  int threads;
+  explicit AppendShares(const AppendArgs& a) {
+    const int heads = (a.q ? a.Hq : 0) + a.Hkv;
+    pairs = a.interleaved ? 0 : a.rotary / 16;
+    singles = a.D / 8 - 2 * pairs;
+    pair_groups = (heads + kPieces / 2 - 1) / (kPieces / 2);
+    single_groups = (heads + kPieces - 1) / kPieces;
+    v_groups = (a.Hkv + kPieces - 1) / kPieces;
+    threads = pairs * pair_groups + singles * single_groups + a.D / 8 * v_groups;
+  }
+};
+
+constexpr int kMostThreads = 128, kCtasPerSm = 8;
+
 template <bool BF16>
-__global__ void __launch_bounds__(512) kv_append_kernel(const __grid_constant__ AppendArgs a, int tokens_per_cta,
-                                                        int* status) {
+__global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
+    kv_append_kernel(const __grid_constant__ AppendArgs a, const __grid_constant__ AppendShares shares, int tokens_per_cta, int slices,
+                     int* status) {
   __shared__ TokenPlace places[kMaxTokens];
-  const int first = blockIdx.x * tokens_per_cta;
+  const int first = blockIdx.x / slices * tokens_per_cta, slice = blockIdx.x % slices;
   const int count = min(tokens_per_cta, a.tokens - first);
   grid_wait_previous();
   grid_allow_next();
-  if (threadIdx.x < count) {
-    const int row = first + threadIdx.x;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, row = first + lane;
     int sequence = row, fresh = 1, index = 0;
-    bool inside = true;
+    bool inside = lane < count;
     if (a.cu_seqlens != nullptr) {
-      // the last sequence that starts at or before this row
-      int low = 0, high = a.batch;
-      while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (ld_global(a.cu_seqlens + mid + 1) <= row) low = mid + 1; else high = mid;
+      sequence = sequence_of(a.cu_seqlens, a.batch, first, lane);
+      if (inside && sequence < a.batch && ld_global(a.cu_seqlens + sequence + 1) <= row) {  // a later sequence begins in between
+        int low = sequence + 1, high = a.batch;
+        while (low < high) {
+          const int mid = (low + high) >> 1;
+          if (ld_global(a.cu_seqlens + mid + 1) <= row) low = mid + 1; else high = mid;
+        }
+        sequence = low;
       }
-      sequence = low;
-      inside = sequence < a.batch;
+      inside = inside && sequence < a.batch;
       if (inside) {
         const int start = ld_global(a.cu_seqlens + sequence);
         fresh = ld_global(a.cu_seqlens + sequence + 1) - start;
@@ -94,85 +138,96 @@ __global__ void __launch_bounds__(512) kv_append_kernel(const __grid_constant__ 
         }
       }
     }
-    places[threadIdx.x] = place;
+    places[lane] = place;
   }
   __syncthreads();
 
-  // This thread's place in a token's row: which tensor, head, and which piece or pair of pieces.
-  const int d8 = a.D / 8, half8 = a.interleaved ? 0 : a.rotary / 16;  // pieces of half the rotated columns
-  const int turned = a.interleaved ? a.rotary / 8 : half8;            // units of a head that the rotation turns
-  const int units = d8 - half8;                                       // of a head of q or k; a head of v has d8
-  int unit = blockIdx.y * blockDim.x + threadIdx.x;
-  const int nq = a.q != nullptr ? a.Hq * units : 0, nk = a.Hkv * units, nv = a.Hkv * d8;
-  if (unit >= nq + nk + nv) return;
-  const bool is_q = unit < nq, is_v = unit >= nq + nk;
-  unit -= is_q ? 0 : (is_v ? nq + nk : nq);
-  const int per_head = is_v ? d8 : units;
-  const int head = unit / per_head;
-  unit -= head * per_head;
-  const bool turns = !is_v && unit < turned, pair = turns && !a.interleaved;
-  const int column = (!is_v && !a.interleaved && unit >= half8 ? unit + half8 : unit) * 8;
-  const void* src = is_q ? a.q : (is_v ? a.v : a.k);
-  const RowStrides ss = is_q ? a.sq : (is_v ? a.sv : a.sk);
-  const long long from = head * ss.head + column;
-  const int other = half8 * 8;  // columns between the two pieces of a pair
-  void* const dense = is_q ? a.q_out : (is_v ? nullptr : a.k_out);
-  const long long dense_row = static_cast<long long>(is_q ? a.Hq : a.Hkv) * a.D;
-  const long long dense_at = static_cast<long long>(head) * a.D + column;
-  void* const cache = is_q ? nullptr : (is_v ? a.v_cache : a.k_cache);
-  const long long cache_at = head * (is_v ? a.sv_cache : a.sk_cache).head + column;
+  // This thread's token among those that the CTA has at a time, and its place in the row.
+  const int at = slice * blockDim.x + threadIdx.x;
+  const int beside = slices > 1 ? 1 : blockDim.x / shares.threads;
+  const int mine = at / shares.threads;
+  if (mine >= beside) return;
+  int unit = at - mine * shares.threads;
+  const int pair_threads = shares.pairs * shares.pair_groups, single_threads = shares.singles * shares.single_groups;
+  const bool pair = unit < pair_threads, is_v = unit >= pair_threads + single_threads;
+  unit -= pair ? 0 : (is_v ? pair_threads + single_threads : pair_threads);
+  const int units = pair ? shares.pairs : (is_v ? a.D / 8 : shares.singles);
+  const int groups = pair ? shares.pair_groups : (is_v ? shares.v_groups : shares.single_groups);
+  const int group = unit / units;
+  unit -= group * units;
+  const int hq = a.q != nullptr ? a.Hq : 0, heads = is_v ? a.Hkv : hq + a.Hkv;
+  const bool turns = pair || (!is_v && a.interleaved && unit < a.rotary / 8);
+  const int column = (pair || is_v ? unit : 2 * shares.pairs + unit) * 8;
+  const int half = a.rotary / 2, angle = pair ? unit * 8 : unit * 4;
 
-#pragma unroll 4
-  for (int t = 0; t < count; ++t) {
+  for (int t = mine; t < count; t += beside) {
     const long long row = first + t;
     const TokenPlace place = places[t];
-    uint4 x = load16(src, row * ss.row + from), y{};
-    if (pair) y = load16(src, row * ss.row + from + other);
-    if (turns && place.position >= 0) {
-      const int half = a.rotary / 2;
-      const float* cos = a.cos + static_cast<long long>(place.position) * half;
-      const float* sin = a.sin + static_cast<long long>(place.position) * half;
-      float f[8], g[8];
-      unpack8<BF16>(x, f);
-      if (pair) {
-        unpack8<BF16>(y, g);
-        const int j = unit * 8;
+    // piece i: which head (below 0: none), and its column
+    auto head_of = [&](int i) {
+      const int head = group + (pair ? i >> 1 : i) * groups;
+      return head < heads ? head : -1;
+    };
+    auto column_of = [&](int i) { return pair && (i & 1) ? column + half : column; };
+    uint4 x[kPieces];
 #pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          const float4 c4 = ld_global(reinterpret_cast<const float4*>(cos + j + i));
-          const float4 s4 = ld_global(reinterpret_cast<const float4*>(sin + j + i));
-          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+    for (int i = 0; i < kPieces; ++i) {
+      const int head = head_of(i);
+      if (head < 0) continue;
+      const bool is_q = !is_v && head < hq;
+      const void* const src = is_v ? a.v : (is_q ? a.q : a.k);
+      const long long row_stride = is_v ? a.sv.row : (is_q ? a.sq.row : a.sk.row), head_stride = is_v ? a.sv.head : (is_q ? a.sq.head : a.sk.head);
+      x[i] = load16(src, row * row_stride + (is_q || is_v ? head : head - hq) * head_stride + column_of(i));
+    }
+    if (turns && place.position >= 0) {
+      const float4* const cos = reinterpret_cast<const float4*>(a.cos + static_cast<long long>(place.position) * half + angle);
+      const float4* const sin = reinterpret_cast<const float4*>(a.sin + static_cast<long long>(place.position) * half + angle);
+      const float4 c0 = ld_global(cos), s0 = ld_global(sin);
+      if (pair) {
+        const float4 c1 = ld_global(cos + 1), s1 = ld_global(sin + 1);
+        const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int i = 0; i < kPieces; i += 2) {
+          float f[8], g[8];
+          unpack8<BF16>(x[i], f);
+          unpack8<BF16>(x[i + 1], g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x1 = f[e], x2 = g[e];
+            f[e] = x1 * c[e] - x2 * s[e];
+            g[e] = x2 * c[e] + x1 * s[e];
+          }
+          x[i] = pack8<BF16>(f);
+          x[i + 1] = pack8<BF16>(g);
+        }
+      } else {
+        const float c[4] = {c0.x, c0.y, c0.z, c0.w}, s[4] = {s0.x, s0.y, s0.z, s0.w};
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          float f[8];
+          unpack8<BF16>(x[i], f);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x1 = f[i + e], x2 = g[i + e];
-            f[i + e] = x1 * c[e] - x2 * s[e];
-            g[i + e] = x2 * c[e] + x1 * s[e];
+            const float x1 = f[2 * e], x2 = f[2 * e + 1];
+            f[2 * e] = x1 * c[e] - x2 * s[e];
+            f[2 * e + 1] = x2 * c[e] + x1 * s[e];
           }
-        }
-        y = pack8<BF16>(g);
-      } else {
-        const int j = unit * 4;
-        const float4 c4 = ld_global(reinterpret_cast<const float4*>(cos + j));
-        const float4 s4 = ld_global(reinterpret_cast<const float4*>(sin + j));
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x1 = f[2 * e], x2 = f[2 * e + 1];
-          f[2 * e] = x1 * c[e] - x2 * s[e];
-          f[2 * e + 1] = x2 * c[e] + x1 * s[e];
+          x[i] = pack8<BF16>(f);
         }
       }
-      x = pack8<BF16>(f);
     }
     const long long slot = is_v ? place.v : place.k;
-    if (cache != nullptr && slot >= 0) {
-      store16(cache, slot + cache_at, x);
-      if (pair) store16(cache, slot + cache_at + other, y);
-    }
-    if (dense != nullptr) {
-      if (slot < 0) x = y = make_uint4(0, 0, 0, 0);
-      store16(dense, row * dense_row + dense_at, x);
-      if (pair) store16(dense, row * dense_row + dense_at + other, y);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int head = head_of(i);
+      if (head < 0) continue;
+      const bool is_q = !is_v && head < hq;
+      const int h = is_q || is_v ? head : head - hq;
+      if (!is_q && slot >= 0)
+        store16(is_v ? a.v_cache : a.k_cache, slot + h * (is_v ? a.sv_cache.head : a.sk_cache.head) + column_of(i), x[i]);
+      void* const dense = is_q ? a.q_out : (is_v ? nullptr : a.k_out);
+      if (dense != nullptr)
+        store16(dense, (row * (is_q ? a.Hq : a.Hkv) + h) * a.D + column_of(i), slot < 0 ? make_uint4(0, 0, 0, 0) : x[i]);
     }
   }
 }
@@ -180,23 +235,18 @@ __global__ void __launch_bounds__(512) kv_append_kernel(const __grid_constant__ 
 }  // namespace
 
 cudaError_t launch_kv_append(const AppendArgs& a, int dtype, int num_sms, int* status, cudaStream_t stream) {
-  const int d8 = a.D / 8, units = d8 - (a.interleaved ? 0 : a.rotary / 16);
-  const int places = (a.q != nullptr ? a.Hq * units : 0) + a.Hkv * (units + d8);
-  const int slices = (places + 511) / 512;                                  // CTAs beside each other on a token
-  const int threads = ((places + slices - 1) / slices + 31) / 32 * 32;
-  const long long wanted = (static_cast<long long>(a.tokens) * slices + 8 * num_sms - 1) / (8ll * num_sms);
-  const int per_cta = static_cast<int>(wanted < 1 ? 1 : (wanted > kMaxTokens ? kMaxTokens : wanted));
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((a.tokens + per_cta - 1) / per_cta, slices);
-  cfg.blockDim = dim3(threads);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return dtype ? cudaLaunchKernelEx(&cfg, kv_append_kernel<true>, a, per_cta, status)
-               : cudaLaunchKernelEx(&cfg, kv_append_kernel<false>, a, per_cta, status);
+  const AppendShares shares(a);
+  const int slices = (shares.threads + kMostThreads - 1) / kMostThreads;  // CTAs beside each other on a token
+  // Tokens that a CTA has at a time: as many as there are threads for, few where there are few, so that every SM has some;
+  // and in all, so that there are several times as many CTAs as run at once.
+  const int fit = slices > 1 ? 1 : kMostThreads / shares.threads, spread = (a.tokens + num_sms - 1) / num_sms;
+  const int beside = std::min({fit, spread, kMaxTokens});
+  const int threads = ((slices > 1 ? (shares.threads + slices - 1) / slices : beside * shares.threads) + 31) / 32 * 32;
+  const int wanted = static_cast<int>((static_cast<long long>(a.tokens) * slices + 48 * num_sms - 1) / (48 * num_sms));
+  const int per_cta = std::min((wanted + beside - 1) / beside * beside, kMaxTokens / beside * beside);
+  const unsigned grid = static_cast<unsigned>((a.tokens + per_cta - 1) / per_cta) * slices;
+  return dtype ? launch_dependent(kv_append_kernel<true>, grid, threads, 0, stream, a, shares, per_cta, slices, status)
+               : launch_dependent(kv_append_kernel<false>, grid, threads, 0, stream, a, shares, per_cta, slices, status);
 }
 
 }  // namespace fa2
