@@ -13,7 +13,7 @@ int check_packed(int rows, int batch, int Hq, int Hkv, int D, int dtype, float s
   if (D > 128) return FA2_ERR_HEAD_DIM;
   if (rows < 0 || rows > (1 << 24) || batch < 1 || batch > (1 << 20)) return FA2_ERR_SHAPE;
   // CTAs of the backward, and the numbers that the forward's CTAs draw
-  if (4ll * packed_capacity(rows, batch) * Hq + 1024 > 0x7fffffffll) return FA2_ERR_SHAPE;
+  if (4ll * packed_capacity(rows, batch) * (Hq + 8) + 1024 > 0x7fffffffll) return FA2_ERR_SHAPE;
   return std::isfinite(scale) && scale > 0.f ? FA2_OK : FA2_ERR_SCALE;
 }
 
@@ -97,7 +97,7 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   const PackedShape s = make_shape(rows, batch, Hq, Hkv, D, dtype, scale);
   const PackedPlan p = packed_plan(const_cast<void*>(plan), rows, batch);
   const PackedStats stats{static_cast<float*>(workspace), static_cast<unsigned*>(workspace) + static_cast<size_t>(p.capacity) * Hq * 256};
-  const int step = packed_step_rows(s, ctx.num_sms);
+  const int step = packed_step_rows(s, Hkv, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
   CUtensorMap tq, tk, tv, tdo, tdq, tdk, tdv;
   if (int e = tq_.map(&tq, rows, D, dtype, step)) return e;
   if (int e = tdo_.map(&tdo, rows, D, dtype, step)) return e;
@@ -109,13 +109,16 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cudaError_t e = launch_packed_preprocess(s, p, cu_seqlens, o, dout, tdo_.st, lse, stats, dq, dk, dv, st)) return static_cast<int>(e);
   if (cudaError_t e = launch_packed_dkdv(s, p, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, step, ctx.status, st)) return static_cast<int>(e);
-  if (step != 128) {  // the other kernel holds Q and dO and walks K and V
+  // the other kernel holds Q and dO and walks K and V
+  if (step != 128) {
     if (int e = tq_.map(&tq, rows, D, dtype, 128)) return e;
     if (int e = tdo_.map(&tdo, rows, D, dtype, 128)) return e;
-    if (int e = tk_.map(&tk, rows, D, dtype, step)) return e;
-    if (int e = tv_.map(&tv, rows, D, dtype, step)) return e;
   }
-  return static_cast<int>(launch_packed_dq(s, p, tq, tk, tv, tdo, tdq, dq, stats, step, ctx.status, st));
+  if (dq_step != 128) {
+    if (int e = tk_.map(&tk, rows, D, dtype, dq_step)) return e;
+    if (int e = tv_.map(&tv, rows, D, dtype, dq_step)) return e;
+  }
+  return static_cast<int>(launch_packed_dq(s, p, tq, tk, tv, tdo, tdq, dq, stats, dq_step, ctx.status, st));
 }
 
 }  // extern "C"

@@ -88,6 +88,28 @@ __device__ int write_list(const int* cu_seqlens, int batch, int per, PackedTile*
   return all;
 }
 
+// The same for up to 32 sequences, one a lane: entry t of a sequence comes behind those of higher numbers in all sequences and
+// those of the same number in the sequences before it, which a warp counts without a word to the others.
+__device__ __forceinline__ int write_short_list(int start, int length, int per, PackedTile* list) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int tiles = (length + 127) >> 7, n = (tiles + per - 1) / per;
+  int base = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, base, o);
+    if (lane >= o) base += y;
+  }
+  base -= tiles;
+  const int most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n));
+  for (int t = warp; t < most; t += warps) {
+    const int higher = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - t - 1, 0)));
+    const unsigned same = __ballot_sync(0xffffffffu, n > t);
+    if (n > t)
+      *reinterpret_cast<int4*>(list + higher + __popc(same & ((1u << lane) - 1u))) = make_int4(start, length, t * per, base);
+  }
+  return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
+}
+
 // Zeros in the rows of a dense [rows, row16 * 8] tensor that no sequence has.
 __device__ void clear_outside(void* out, long long row16, int first, int last, int rows, long long worker, long long workers) {
   if (out == nullptr) return;
@@ -102,6 +124,22 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
   __shared__ int full[kBins], rest[kBins], cursor[kBins], shared[32], longest;
   grid_wait_previous();
   grid_allow_next();
+  if (blockIdx.x == 0 && batch <= 32) {
+    const int lane = threadIdx.x & 31;
+    const int start = lane < batch ? ld_global(cu_seqlens + lane) : 0, end = lane < batch ? ld_global(cu_seqlens + lane + 1) : 0;
+    const bool ok = __all_sync(0xffffffffu, start >= 0 && end >= start && end <= rows);
+    int counts[2] = {0, 0};
+    if (ok) {
+      counts[0] = write_short_list(start, end - start, 1, plan.tiles);
+      if (pairs) counts[1] = write_short_list(start, end - start, 2, plan.pairs);
+    }
+    if (threadIdx.x == 0) {
+      plan.counts[0] = counts[0];
+      plan.counts[1] = counts[1];
+      if (!ok) atomicCAS(status, 0, kStatusSequences);
+    }
+    return;
+  }
   const bool ok = sequences_ok(cu_seqlens, batch, rows);
   if (blockIdx.x > 0) {
     const int first = ok ? ld_global(cu_seqlens) : rows, last = ok ? ld_global(cu_seqlens + batch) : rows;
@@ -131,12 +169,12 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
 
 // ----------------------------------------------------------------------------------------
 // Backward preprocess: delta = rowsum(dO o O), with -lse log2(e) by tile.  Bound by reading O and dO once.  A CTA takes
-// 32 rows of a tile with all of their heads, which lie one behind the other in memory; D / 8 adjacent lanes add up
+// eight heads of 32 rows of a tile, which lie one behind the other in memory; D / 8 adjacent lanes add up
 // one head of one row in a fixed order.
 // ----------------------------------------------------------------------------------------
 constexpr int kPreThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPreHeads = 64;  // heads whose results shared memory holds
+constexpr int kPreHeads = 8;  // of a CTA
 
 template <bool BF16>
 __device__ __forceinline__ float2 both(uint32_t v) {
@@ -153,6 +191,7 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
   __shared__ unsigned amax[kPreHeads];
   grid_wait_previous();
   grid_allow_next();
+  int entry, part;
   // rows of the gradients that no sequence has
   {
     const int count = ld_global(counts);
@@ -161,66 +200,67 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
     clear_outside(dq, static_cast<long long>(Hq) * Dg / 8, first, last, rows, worker, workers);
     clear_outside(dk, static_cast<long long>(Hkv) * Dg / 8, first, last, rows, worker, workers);
     clear_outside(dv, static_cast<long long>(Hkv) * Dg / 8, first, last, rows, worker, workers);
-    if (static_cast<int>(blockIdx.x >> 2) >= count) return;
+    const int parts = 4 * ((Hq + kPreHeads - 1) / kPreHeads);  // CTAs of a tile
+    entry = blockIdx.x / parts, part = blockIdx.x - entry * parts;
+    if (entry >= count) return;
   }
-  const PackedTile e = load_tile(tiles + (blockIdx.x >> 2));
-  const int quarter = blockIdx.x & 3;
+  const PackedTile e = load_tile(tiles + entry);
+  const int quarter = part & 3, h0 = part / 4 * kPreHeads, heads = min(Hq - h0, kPreHeads);
   const int local = e.tile * 128 + quarter * 32;  // first of the 32 rows in the sequence
   const int here = min(max(e.length - local, 0), 32);
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, G = Hq / Hkv;
-  for (int h0 = 0; h0 < Hq; h0 += kPreHeads) {
-    const int heads = min(Hq - h0, kPreHeads);
-    if (threadIdx.x < kPreHeads) amax[threadIdx.x] = 0;
-    __syncthreads();
-    const int work = here * heads;
-    for (int i0 = group; i0 < (work + 4 * kGroups - 1) / (4 * kGroups) * (4 * kGroups); i0 += 4 * kGroups) {
-      uint4 a[4], b[4];
+  if (threadIdx.x < kPreHeads) amax[threadIdx.x] = 0;
+  // the result that this thread writes at the end
+  static_assert(kPreHeads * 32 == kPreThreads, "one result a thread");
+  const int out_h = threadIdx.x / 32, out_r = threadIdx.x % 32;
+  const bool writes = out_h < heads, inside = writes && out_r < here;
+  const float row_lse = inside ? ld_global(lse + static_cast<size_t>(h0 + out_h) * rows + e.row0 + local + out_r) : 0.f;
+  __syncthreads();
+  const int work = here * heads;
+  for (int i0 = group; i0 < (work + 4 * kGroups - 1) / (4 * kGroups) * (4 * kGroups); i0 += 4 * kGroups) {
+    uint4 a[4], b[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kGroups, r = i / heads, h = h0 + i - r * heads;
-        a[u] = b[u] = make_uint4(0, 0, 0, 0);
-        if (i < work && lane * 8 < Dg) {
-          const long long row = e.row0 + local + r;
-          a[u] = ld_global(reinterpret_cast<const uint4*>(o + (row * Hq + h) * Dg + lane * 8));
-          b[u] = ld_global(reinterpret_cast<const uint4*>(dout + row * sdo.row + h * sdo.head + lane * 8));
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kGroups, r = i / heads, h = i - r * heads;
-        const uint32_t x[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, y[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
-        float sum = 0.f;
-        unsigned most = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float2 f = both<BF16>(x[w]), g = both<BF16>(y[w]);
-          sum = fmaf(f.x, g.x, sum);
-          sum = fmaf(f.y, g.y, sum);
-          if constexpr (!BF16) most = max(most, max(y[w] & 0x7fffu, (y[w] >> 16) & 0x7fffu));
-        }
-#pragma unroll
-        for (int s = kLanes / 2; s > 0; s >>= 1) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, s);
-          if constexpr (!BF16) most = max(most, __shfl_xor_sync(0xffffffffu, most, s));
-        }
-        if (lane == 0 && i < work) {
-          delta[h][r] = sum;
-          if constexpr (!BF16) atomicMax(amax + h, most);
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kGroups, r = i / heads, h = h0 + i - r * heads;
+      a[u] = b[u] = make_uint4(0, 0, 0, 0);
+      if (i < work && lane * 8 < Dg) {
+        const long long row = e.row0 + local + r;
+        a[u] = ld_global(reinterpret_cast<const uint4*>(o + (row * Hq + h) * Dg + lane * 8));
+        b[u] = ld_global(reinterpret_cast<const uint4*>(dout + row * sdo.row + h * sdo.head + lane * 8));
       }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * 32; i += kPreThreads) {
-      const int h = h0 + i / 32, r = i % 32;
-      float* const to = out.stats + (static_cast<size_t>(h) * capacity + e.base + e.tile) * 256 + quarter * 32 + r;
-      const bool inside = r < here;
-      to[0] = inside ? -ld_global(lse + static_cast<size_t>(h) * rows + e.row0 + local + r) * kLog2e : -INFINITY;
-      to[128] = inside ? -delta[i / 32][r] : 0.f;
-      if (!BF16 && r == 0)
-        out.amax[((static_cast<size_t>(h / G) * capacity + e.base + e.tile) * 4 + quarter) * G + h % G] = amax[i / 32];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * kGroups, r = i / heads, h = i - r * heads;
+      const uint32_t x[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, y[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+      float sum = 0.f;
+      unsigned most = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 f = both<BF16>(x[w]), g = both<BF16>(y[w]);
+        sum = fmaf(f.x, g.x, sum);
+        sum = fmaf(f.y, g.y, sum);
+        if constexpr (!BF16) most = max(most, max(y[w] & 0x7fffu, (y[w] >> 16) & 0x7fffu));
+      }
+#pragma unroll
+      for (int s = kLanes / 2; s > 0; s >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        if constexpr (!BF16) most = max(most, __shfl_xor_sync(0xffffffffu, most, s));
+      }
+      if (lane == 0 && i < work) {
+        delta[h][r] = sum;
+        if constexpr (!BF16) atomicMax(amax + h, most);
+      }
     }
-    __syncthreads();
   }
+  __syncthreads();
+  if (!writes) return;
+  const int h = h0 + out_h;
+  float* const to = out.stats + (static_cast<size_t>(h) * capacity + e.base + e.tile) * 256 + quarter * 32 + out_r;
+  to[0] = inside ? -row_lse * kLog2e : -INFINITY;
+  to[128] = inside ? -delta[out_h][out_r] : 0.f;
+  if (!BF16 && out_r == 0)
+    out.amax[((static_cast<size_t>(h / G) * capacity + e.base + e.tile) * 4 + quarter) * G + h % G] = amax[out_h];
 }
 
 }  // namespace
@@ -239,7 +279,7 @@ static cudaError_t launch_preprocess_t(const PackedShape& s, const PackedPlan& p
                                        const void* dout, const RowStrides& sdo, const float* lse, const PackedStats& stats,
                                        void* dq, void* dk, void* dv, cudaStream_t stream) {
   auto kern = s.dtype ? packed_preprocess_kernel<D, true> : packed_preprocess_kernel<D, false>;
-  return launch_dependent(kern, 4u * plan.capacity, kPreThreads, 0, stream, plan.tiles, plan.counts, plan.capacity, cu_seqlens,
+  return launch_dependent(kern, 4u * plan.capacity * ((s.Hq + kPreHeads - 1) / kPreHeads), kPreThreads, 0, stream, plan.tiles, plan.counts, plan.capacity, cu_seqlens,
                           static_cast<const uint16_t*>(o), static_cast<const uint16_t*>(dout), sdo, lse, stats, s.rows, s.batch, s.Hq,
                           s.Hkv, s.Dg, dq, dk, dv);
 }

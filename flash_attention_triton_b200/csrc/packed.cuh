@@ -70,8 +70,8 @@ cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, cons
 cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& plan, const int* cu_seqlens, const void* o,
                                      const void* dout, const RowStrides& sdo, const float* lse, const PackedStats& stats,
                                      void* dq, void* dk, void* dv, cudaStream_t stream);
-// Rows of a step of the backward kernels, and the box height of the tensors they walk.
-int packed_step_rows(const PackedShape& s, int num_sms);
+// Rows of a step of a backward kernel with `heads` CTAs to a tile, and the box height of the tensors it walks.
+int packed_step_rows(const PackedShape& s, int heads, int num_sms);
 cudaError_t launch_packed_dkdv(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                                const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                                void* dk, void* dv, const PackedStats& stats, int step_rows, int* status, cudaStream_t stream);

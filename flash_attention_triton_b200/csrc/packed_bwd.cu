@@ -632,8 +632,10 @@ cudaError_t launch_dq_t(const PackedShape& s, const PackedPlan& plan, const CUte
 
 }  // namespace
 
-int packed_step_rows(const PackedShape& s, int num_sms) {
-  return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * s.Hkv >= 330ll * num_sms ? 64 : 128;
+// 64 (two CTAs on an SM) up to head dim 64, once there are CTAs to pair: the line of bwd_step_rows (common.cuh) for tiles of
+// middling sequences, on the number of tiles that the rows have at most.
+int packed_step_rows(const PackedShape& s, int heads, int num_sms) {
+  return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * heads >= 300ll * num_sms ? 64 : 128;
 }
 
 #define FA2_DTYPES(CALL, DD, KK, WW) return s.dtype ? CALL<DD, true, KK, WW>(FA2_ARGS) : CALL<DD, false, KK, WW>(FA2_ARGS)
