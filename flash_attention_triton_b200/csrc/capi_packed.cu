@@ -97,7 +97,8 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   const PackedShape s = make_shape(rows, batch, Hq, Hkv, D, dtype, scale);
   const PackedPlan p = packed_plan(const_cast<void*>(plan), rows, batch);
   const PackedStats stats{static_cast<float*>(workspace), static_cast<unsigned*>(workspace) + static_cast<size_t>(p.capacity) * Hq * 256};
-  const int step = packed_step_rows(s, Hkv, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
+  const int cluster = packed_cluster(s, ctx.num_sms);
+  const int step = packed_step_rows(s, Hkv * cluster, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
   CUtensorMap tq, tk, tv, tdo, tdq, tdk, tdv;
   if (int e = tq_.map(&tq, rows, D, dtype, step)) return e;
   if (int e = tdo_.map(&tdo, rows, D, dtype, step)) return e;
@@ -108,7 +109,7 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   if (int e = tdv_.map(&tdv, rows, D, dtype, 32)) return e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cudaError_t e = launch_packed_preprocess(s, p, cu_seqlens, o, dout, tdo_.st, lse, stats, dq, dk, dv, st)) return static_cast<int>(e);
-  if (cudaError_t e = launch_packed_dkdv(s, p, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, step, ctx.status, st)) return static_cast<int>(e);
+  if (cudaError_t e = launch_packed_dkdv(s, p, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, step, cluster, ctx.status, st)) return static_cast<int>(e);
   // the other kernel holds Q and dO and walks K and V
   if (step != 128) {
     if (int e = tq_.map(&tq, rows, D, dtype, 128)) return e;

@@ -72,12 +72,34 @@ cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& pla
                                      void* dq, void* dk, void* dv, cudaStream_t stream);
 // Rows of a step of a backward kernel with `heads` CTAs to a tile, and the box height of the tensors it walks.
 int packed_step_rows(const PackedShape& s, int heads, int num_sms);
+// CTAs of the dK / dV kernel that share the query heads of a KV tile: 1, or 2 where G is even.
+int packed_cluster(const PackedShape& s, int num_sms);
 cudaError_t launch_packed_dkdv(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                                const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
-                               void* dk, void* dv, const PackedStats& stats, int step_rows, int* status, cudaStream_t stream);
+                               void* dk, void* dv, const PackedStats& stats, int step_rows, int cluster, int* status,
+                               cudaStream_t stream);
 cudaError_t launch_packed_dq(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                              const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdq, void* dq,
                              const PackedStats& stats, int step_rows, int* status, cudaStream_t stream);
+
+// launch_dependent (common.cuh) in clusters of `cluster` CTAs.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_dependent_cluster(void (*kernel)(Params...), unsigned grid, unsigned cluster, int threads, int smem_bytes,
+                                            cudaStream_t stream, Args&&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 
 #ifdef __CUDACC__
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {

@@ -12,30 +12,50 @@ namespace fa2 {
 namespace {
 
 // 32 rows of a warp from a [128, KD] fp32 accumulator as 16 bits, times `mul`: through a free tile buffer and the tensor map
-// where all 32 belong to the sequence (`left` >= 32), row by row where only the first `left` do.
+// where all 32 belong to the sequence (`left` >= 32), row by row where only the first `left` do.  `parts` of the same rows
+// from other CTAs, `part_stride` floats apart, are added first: [KD / 4][32 lanes][4] floats each.
 template <int D, bool BF16, int KD>
 __device__ __forceinline__ void store_packed_rows(uint32_t tmem_row_addr, uint8_t* stage, int warp4, int lane,
                                                   const CUtensorMap* map, int row, int head, int heads, int left, void* out,
-                                                  int cols, float mul) {
-  if (left >= 32) {
-    store_rows_16bit<D, BF16, KD>(tmem_row_addr, stage, warp4, lane, map, row - warp4 * 32, HeadCoord{head, 0}, row + 32, mul);
-    return;
-  }
+                                                  int cols, float mul, const float* part = nullptr, int parts = 0,
+                                                  int part_stride = 0) {
+  using T = Tile<D>;
+  const bool whole = left >= 32;
   uint16_t* const dst = static_cast<uint16_t*>(out) + (static_cast<long long>(row + lane) * heads + head) * cols;
 #pragma unroll
   for (int c0 = 0; c0 < KD; c0 += 32) {
     uint32_t v[32];
     tmem_ld_x32(tmem_row_addr + c0, v);
     tmem_wait_ld();
+    float* const f = reinterpret_cast<float*>(v);
+    for (int i = 0; i < parts; ++i)
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float4 x = reinterpret_cast<const float4*>(part + i * part_stride)[(c0 / 4 + p) * 32 + lane];
+        f[4 * p] += x.x, f[4 * p + 1] += x.y, f[4 * p + 2] += x.z, f[4 * p + 3] += x.w;
+      }
+    const int piece0 = (c0 % T::kChunkElems) / 8;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       uint4 val;
-      val.x = pack2<BF16>(__uint_as_float(v[8 * p + 0]) * mul, __uint_as_float(v[8 * p + 1]) * mul);
-      val.y = pack2<BF16>(__uint_as_float(v[8 * p + 2]) * mul, __uint_as_float(v[8 * p + 3]) * mul);
-      val.z = pack2<BF16>(__uint_as_float(v[8 * p + 4]) * mul, __uint_as_float(v[8 * p + 5]) * mul);
-      val.w = pack2<BF16>(__uint_as_float(v[8 * p + 6]) * mul, __uint_as_float(v[8 * p + 7]) * mul);
-      if (lane < left && c0 + 8 * p < cols) *reinterpret_cast<uint4*>(dst + c0 + 8 * p) = val;
+      val.x = pack2<BF16>(f[8 * p + 0] * mul, f[8 * p + 1] * mul);
+      val.y = pack2<BF16>(f[8 * p + 2] * mul, f[8 * p + 3] * mul);
+      val.z = pack2<BF16>(f[8 * p + 4] * mul, f[8 * p + 5] * mul);
+      val.w = pack2<BF16>(f[8 * p + 6] * mul, f[8 * p + 7] * mul);
+      if (whole)
+        *reinterpret_cast<uint4*>(stage + c0 / T::kChunkElems * T::kChunkTileBytes + swizzled_offset<D>(warp4 * 32 + lane, piece0 + p)) = val;
+      else if (lane < left && c0 + 8 * p < cols)
+        *reinterpret_cast<uint4*>(dst + c0 + 8 * p) = val;
     }
+  }
+  if (!whole) return;
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    for (int ch = 0; ch < (KD + T::kChunkElems - 1) / T::kChunkElems; ++ch)
+      tma_store_4d(map, ch * T::kChunkElems, row, HeadCoord{head, 0}, smem_u32(stage + ch * T::kChunkTileBytes + warp4 * 32 * T::kRowBytes));
+    tma_store_commit();
+    tma_store_wait_all();
   }
 }
 
@@ -53,9 +73,13 @@ __device__ __forceinline__ float group_dscale(const PackedStats& stats, int capa
 }
 
 // =========================================================================================
-// dK / dV: one CTA per KV tile of a key head
+// dK / dV: one CTA per KV tile of a key head, or a cluster of two (S) that share its query heads
 // =========================================================================================
-template <int D, bool BF16, int KD, int W>
+// A KV tile with G query heads is G times the work of one, and there are G times fewer of them, so with few tiles a launch
+// waits for the longest of them.  The CTAs of a cluster then take half of the query heads each.  At their end each sends
+// its fp32 accumulators of the half of the 128 rows that the other one owns into that one's idle rings: no memory, no
+// other launch, one order of the sum.  When: packed_cluster.
+template <int D, bool BF16, int KD, int W, int S>
 __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::kCtasPerSm)
     packed_dkdv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                        const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
@@ -93,7 +117,9 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
   grid_wait_previous();
   grid_allow_next();
 
-  const int entry = blockIdx.x / Hkv, kv_head = blockIdx.x - entry * Hkv;
+  static_assert(S == 1 || S == 2, "packed_cluster");
+  const int rank = S == 1 ? 0 : blockIdx.x % S, entry = blockIdx.x / S / Hkv, kv_head = blockIdx.x / S - entry * Hkv;
+  const int first_head = kv_head * G + rank * (G / S);  // of this CTA's query heads
   if (entry < ld_global(counts)) {
   const PackedTile e = load_tile(list + entry);
   const int ntiles = (e.length + 127) >> 7;
@@ -101,7 +127,7 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
   const int row_k = e.row0 + jt * 128, left = e.length - jt * 128;  // rows of the KV tile in the sequence
   // A Q tile is worked through in kSub steps of W rows, first rows first (dkdv_roles).
   constexpr int kSub = 128 / W;
-  const int per_head = nq * kSub, nsteps = per_head * G;
+  const int per_head = nq * kSub, nsteps = per_head * (G / S);
   const HeadCoord hk{kv_head, 0};
   // step u of a query head: first row in the sequence
   auto q_row = [&](int u) { return (ntiles - 1 - u / kSub) * 128 + (u % kSub) * W; };
@@ -121,8 +147,8 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
       }
       int s = 0, ph = 1;
       bool ok = true;
-      for (int g = 0; ok && g < G; ++g) {
-        const HeadCoord hq{kv_head * G + g, 0};
+      for (int g = 0; ok && g < G / S; ++g) {
+        const HeadCoord hq{first_head + g, 0};
         const float* head_stats = stats.stats + (static_cast<size_t>(hq.h) * capacity + e.base) * 256;
         for (int u = 0; u < per_head; ++u) {
           const int row = q_row(u);
@@ -229,6 +255,10 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
       }
     }
     __syncwarp();
+    if constexpr (S > 1) {
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     // ---------------------------------------------------------------- compute groups
     reg_inc<C::kComputeRegs>();
@@ -299,16 +329,35 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::kBarDsReady));
     }
-    // epilogue: group 0 stores dV, group 1 stores dK, staged through the idle dO / Q buffers
-    if (ok && mbar_wait_warp(bar(C::kBarDone), 0, w, kBSiteCmpDone)) {
-      tc_fence_after();
-      if (wg == 0)
-        store_packed_rows<D, BF16, KD>(tmem_base + lane_base + C::kColDV, smem + C::kOffDO, w4, lane, &tdv, row_k + w4 * 32, kv_head,
-                                       Hkv, left - w4 * 32, dv, cols, 1.0f);
-      else
-        store_packed_rows<D, BF16, KD>(tmem_base + lane_base + C::kColDK, smem + C::kOffQ, w4, lane, &tdk, row_k + w4 * 32, kv_head,
-                                       Hkv, left - w4 * 32, dk, cols, inv_dscale);
+    // epilogue: group 0 has dV, group 1 dK; staged through the idle V and K tiles
+    ok = ok && mbar_wait_warp(bar(C::kBarDone), 0, w, kBSiteCmpDone);
+    tc_fence_after();
+    const uint32_t sums = tmem_base + lane_base + (wg == 0 ? C::kColDV : C::kColDK);
+    constexpr int kWarpsOfRank = 4 / S, kPartFloats = KD * 32;  // warps of a group whose rows a CTA owns; floats of 32 rows
+    const int owner = w4 / kWarpsOfRank;
+    // parts that arrive here: [sender, without the receiver][dV, dK][warp of the owner][KD / 4][32 lanes][4]
+    const int at = (wg * kWarpsOfRank + w4 % kWarpsOfRank) * kPartFloats;
+    constexpr int kSenderFloats = 2 * kWarpsOfRank * kPartFloats;
+    static_assert(S == 1 || (S - 1) * kSenderFloats * 4 <= 2 * C::kStages * C::kStepBytes, "the rings take the parts");
+    if constexpr (S > 1) {
+      cluster_sync();  // every CTA has formed its last product: the rings are idle
+      if (ok && owner != rank) {
+        const uint32_t to = cluster_address(smem_base + C::kOffQ + ((rank < owner ? rank : rank - 1) * kSenderFloats + at) * 4, owner);
+#pragma unroll
+        for (int c0 = 0; c0 < KD; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld_x32(sums + c0, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int p = 0; p < 8; ++p) st_cluster_v4(to + ((c0 / 4 + p) * 32 + lane) * 16, v + 4 * p);
+        }
+      }
+      cluster_sync();
     }
+    if (ok && owner == rank)
+      store_packed_rows<D, BF16, KD>(sums, smem + (wg == 0 ? C::kOffV : C::kOffK), w4, lane, wg == 0 ? &tdv : &tdk, row_k + w4 * 32,
+                                     kv_head, Hkv, left - w4 * 32, wg == 0 ? dv : dk, cols, wg == 0 ? 1.0f : inv_dscale,
+                                     reinterpret_cast<const float*>(smem + C::kOffQ) + at, S - 1, kSenderFloats);
   }
   }
 
@@ -605,17 +654,24 @@ __global__ void __launch_bounds__(PackedDqCfg<D, W>::kThreads, PackedDqCfg<D, W>
   }
 }
 
-template <int D, bool BF16, int KD, int W>
-cudaError_t launch_dkdv_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+template <int D, bool BF16, int KD, int W, int S>
+cudaError_t launch_dkdv_s(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                           const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                           void* dk, void* dv, const PackedStats& stats, int* status, cudaStream_t stream) {
   using C = DkdvCfg<D, 0, W>;
-  auto kern = packed_dkdv_kernel<D, BF16, KD, W>;
+  auto kern = packed_dkdv_kernel<D, BF16, KD, W, S>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kern, static_cast<unsigned>(plan.capacity) * s.Hkv, C::kThreads, C::kSmemBytes, stream, tq, tk, tv, tdo, tdk,
-                          tdv, dk, dv, plan.tiles, plan.counts, stats, plan.capacity, s.Hkv, s.Hq / s.Hkv, s.Dg, s.scale,
-                          s.scale * 1.4426950408889634f, status);
+  return launch_dependent_cluster(kern, static_cast<unsigned>(plan.capacity) * s.Hkv * S, S, C::kThreads, C::kSmemBytes, stream, tq, tk, tv,
+                                  tdo, tdk, tdv, dk, dv, plan.tiles, plan.counts, stats, plan.capacity, s.Hkv, s.Hq / s.Hkv, s.Dg, s.scale,
+                                  s.scale * 1.4426950408889634f, status);
+}
+template <int D, bool BF16, int KD, int W>
+cudaError_t launch_dkdv_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+                          const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
+                          void* dk, void* dv, const PackedStats& stats, int cluster, int* status, cudaStream_t stream) {
+  if (cluster == 2) return launch_dkdv_s<D, BF16, KD, W, 2>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
+  return launch_dkdv_s<D, BF16, KD, W, 1>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
 }
 template <int D, bool BF16, int KD, int W>
 cudaError_t launch_dq_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
@@ -638,6 +694,15 @@ int packed_step_rows(const PackedShape& s, int heads, int num_sms) {
   return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * heads >= 300ll * num_sms ? 64 : 128;
 }
 
+// Two where single CTAs would not fill the SMs one and a half times.  Whole backward, microseconds, clusters of 1 / 2 / 4:
+//   41 CTAs (16 x 200 rows, 8 / 1 heads of 128) 65.8 / 58.6 / 59.0, 130 (8192, 8 / 2 of 128) 669 / 386 / 468,
+//   192 (eight of 256 to 1024, 16 / 4 of 64) 83.3 / 74.6 / 79.0, 260 (8192, 16 / 4 of 128) 840 / 841 / 929,
+//   264 (2 x 4096, 16 / 4 of 64) 301 / 291 / 310, 272 (2 x 2048, 32 / 8 of 128) 276 / 290 / 343, 576 (8 x 1024, 32 / 8 of 128) 323 / 410 / 499.
+int packed_cluster(const PackedShape& s, int num_sms) {
+  const long long ctas = static_cast<long long>(packed_capacity(s.rows, s.batch)) * s.Hkv;
+  return s.Hq / s.Hkv % 2 == 0 && 2 * ctas <= 3ll * num_sms ? 2 : 1;
+}
+
 #define FA2_DTYPES(CALL, DD, KK, WW) return s.dtype ? CALL<DD, true, KK, WW>(FA2_ARGS) : CALL<DD, false, KK, WW>(FA2_ARGS)
 #define FA2_DISPATCH(CALL)                                        \
   if (s.D == 32 && step_rows == 64) FA2_DTYPES(CALL, 32, 32, 64); \
@@ -649,8 +714,8 @@ int packed_step_rows(const PackedShape& s, int heads, int num_sms) {
 
 cudaError_t launch_packed_dkdv(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                                const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
-                               void* dk, void* dv, const PackedStats& stats, int step_rows, int* status, cudaStream_t stream) {
-#define FA2_ARGS s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream
+                               void* dk, void* dv, const PackedStats& stats, int step_rows, int cluster, int* status, cudaStream_t stream) {
+#define FA2_ARGS s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, cluster, status, stream
   FA2_DISPATCH(launch_dkdv_t);
 #undef FA2_ARGS
 }

@@ -170,6 +170,22 @@ __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
 }
 
 // ----------------------------------------------------------------------------------------
+// Thread-block clusters: a meeting of all threads of all CTAs (converged warps), which makes what they wrote before
+// visible, and stores to another CTA's shared memory.
+// ----------------------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_address(uint32_t smem_addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+
+// ----------------------------------------------------------------------------------------
 // TMA: tiled 4-D tensor copies, coordinates {x = element in row, y = row, head, batch}.
 // Batch and head are separate dimensions so that the tensors may have any batch / head /
 // row strides (multiples of 16 bytes); boxes are always one head of one batch wide.
