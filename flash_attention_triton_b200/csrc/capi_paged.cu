@@ -83,7 +83,10 @@ int fa2_decode(const void* q, const void* k_cache, const void* v_cache, void* ou
   if (!q || !k_cache || !v_cache || !out || !block_table || !lengths) return FA2_ERR_NULL_POINTER;
   if (int e = check_heads(Hq, Hkv, D, dtype)) return e;
   if (int e = check_cache(batch, pages, page_size, table_width)) return e;
-  if (static_cast<long long>(batch) * Hq > 0x7fffffffll) return FA2_ERR_SHAPE;
+  // query heads of the call; the units of 64 keys that its CTAs share out
+  if (static_cast<long long>(batch) * Hq > 0x7fffffffll ||
+      (static_cast<long long>(table_width) * page_size / 64 + 3) * batch > 0x7fffffffll / Hkv)
+    return FA2_ERR_SHAPE;
   for (const void* p : {q, k_cache, v_cache, static_cast<const void*>(out), static_cast<const void*>(workspace)})
     if (!aligned_to(p, 16)) return FA2_ERR_MISALIGNED;
   if (!std::isfinite(scale) || !(scale > 0.f)) return FA2_ERR_SCALE;

@@ -100,7 +100,7 @@ def test_workspace_size():
 
 @pytest.mark.parametrize("change,code", [
     ({"q": 0}, -1), ({"table": 0}, -1), ({"D": 12}, -2), ({"dtype": 2}, -3), ({"q": 0x1008}, -4), ({"batch": 0}, -5),
-    ({"width": 1 << 30}, -5), ({"scale": math.inf}, -9), ({"bytes": 16}, -10), ({"Hq": 7}, -13),
+    ({"width": 1 << 30}, -5), ({"width": 1 << 26, "batch": 200}, -5), ({"scale": math.inf}, -9), ({"bytes": 16}, -10), ({"Hq": 7}, -13),
     ({"strides": [128, 64, 2048, 128, 60, 2048, 128, 64, 4]}, -12), ({"strides": [128, 32, 2048, 128, 64, 2048, 128, 64, 4]}, -12),
 ])
 def test_decode_codes(change, code):
