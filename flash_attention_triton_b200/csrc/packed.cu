@@ -191,20 +191,20 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
   __shared__ unsigned amax[kPreHeads];
   grid_wait_previous();
   grid_allow_next();
-  int entry, part;
+  const int parts = 4 * ((Hq + kPreHeads - 1) / kPreHeads);  // CTAs of a tile
+  const int entry = blockIdx.x / parts, part = blockIdx.x - entry * parts;
+  // (asked for together: an entry behind the last one may hold anything)
+  const int count = ld_global(counts), start = ld_global(cu_seqlens), end = ld_global(cu_seqlens + batch);
+  const PackedTile e = load_tile(tiles + entry);
   // rows of the gradients that no sequence has
   {
-    const int count = ld_global(counts);
-    const int first = count ? ld_global(cu_seqlens) : rows, last = count ? ld_global(cu_seqlens + batch) : rows;
+    const int first = count ? start : rows, last = count ? end : rows;
     const long long worker = static_cast<long long>(blockIdx.x) * kPreThreads + threadIdx.x, workers = static_cast<long long>(gridDim.x) * kPreThreads;
     clear_outside(dq, static_cast<long long>(Hq) * Dg / 8, first, last, rows, worker, workers);
     clear_outside(dk, static_cast<long long>(Hkv) * Dg / 8, first, last, rows, worker, workers);
     clear_outside(dv, static_cast<long long>(Hkv) * Dg / 8, first, last, rows, worker, workers);
-    const int parts = 4 * ((Hq + kPreHeads - 1) / kPreHeads);  // CTAs of a tile
-    entry = blockIdx.x / parts, part = blockIdx.x - entry * parts;
-    if (entry >= count) return;
   }
-  const PackedTile e = load_tile(tiles + entry);
+  if (entry >= count) return;
   const int quarter = part & 3, h0 = part / 4 * kPreHeads, heads = min(Hq - h0, kPreHeads);
   const int local = e.tile * 128 + quarter * 32;  // first of the 32 rows in the sequence
   const int here = min(max(e.length - local, 0), 32);
