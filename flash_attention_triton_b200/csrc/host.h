@@ -44,7 +44,8 @@ inline double scale_argument(PyObject* arg, int64_t head_dim) {
 // Kernels read a [rows, H, D] tensor through its own strides: unit last stride, 16-byte aligned base, row and head
 // strides that are multiples of 8 elements and at least D (those of dimensions of size 1 do not matter).
 bool rows_readable(const at::Tensor& t);
-inline at::Tensor rows_input(const at::Tensor& t) { return rows_readable(t) ? t : t.contiguous(); }
+// What cannot be read so is copied (a tensor that is dense but not aligned, too).
+inline at::Tensor rows_input(const at::Tensor& t) { return rows_readable(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 // AssertionError as flash_attention_v2 raises it, for what is not a CUDA tensor; ValueError for another device.
 void check_devices(std::initializer_list<std::pair<const at::Tensor*, const char*>> tensors);

@@ -136,6 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
     if (threadIdx.x == 0) {
       plan.counts[0] = counts[0];
       plan.counts[1] = counts[1];
+    plan.counts[2] = 0;
       if (!ok) atomicCAS(status, 0, kStatusSequences);
     }
     return;
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
   if (threadIdx.x == 0) {
     plan.counts[0] = counts[0];
     plan.counts[1] = counts[1];
+    plan.counts[2] = 0;
     if (!ok) atomicCAS(status, 0, kStatusSequences);
   }
 }

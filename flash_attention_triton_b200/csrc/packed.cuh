@@ -27,7 +27,7 @@ struct PackedTile {
 };
 
 struct PackedPlan {
-  int* counts;         // [0] tiles, [1] pairs of tiles
+  int* counts;         // [0] tiles, [1] pairs of tiles, [2] the forward's work counter, zero behind the plan kernel
   PackedTile* tiles;   // heaviest first, room for `capacity`
   PackedTile* pairs;   // pairs of adjacent tiles, likewise
   int capacity;
@@ -65,7 +65,7 @@ constexpr int kStatusSequences = 0x80000;
 cudaError_t launch_packed_plan(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, bool pairs, void* out,
                                int* status, int num_sms, cudaStream_t stream);
 cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
-                              const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, const LaunchCtx& ctx,
+                              const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms,
                               cudaStream_t stream);
 cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& plan, const int* cu_seqlens, const void* o,
                                      const void* dout, const RowStrides& sdo, const float* lse, const PackedStats& stats,

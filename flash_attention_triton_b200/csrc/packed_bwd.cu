@@ -688,10 +688,11 @@ cudaError_t launch_dq_t(const PackedShape& s, const PackedPlan& plan, const CUte
 
 }  // namespace
 
-// 64 (two CTAs on an SM) up to head dim 64, once there are CTAs to pair: the line of bwd_step_rows (common.cuh) for tiles of
-// middling sequences, on the number of tiles that the rows have at most.
+// 64 (two CTAs on an SM) up to head dim 64, once there are CTAs to pair (DkdvCfg in bwd_roles.cuh), by the tiles that the rows
+// have at most.  Whole backward, fp16, head dim 64, microseconds with the line at 100 / 200 / 300 CTAs a hundred SMs / none:
+// 2 x 2048 rows, 16 / 4 heads 119 / 97 / 98 / 103, 4 x 1024 74 / 67 / 66 / 74, 32 x 300, 8 / 2 heads 62 / 60 / 67 / 79.
 int packed_step_rows(const PackedShape& s, int heads, int num_sms) {
-  return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * heads >= 300ll * num_sms ? 64 : 128;
+  return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * heads >= 200ll * num_sms ? 64 : 128;
 }
 
 // Two where single CTAs would not fill the SMs one and a half times.  Whole backward, microseconds, clusters of 1 / 2 / 4:

@@ -68,8 +68,8 @@ template <int D, bool BF16, int KD>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, uint16_t* out, float* lse,
-                      const int* counts, const PackedTile* list, int rows, int Hq, int G, int cols, bool two_heads,
-                      float scale_log2, int* status, unsigned int* work_counter) {
+                      int* counts, const PackedTile* list, int rows, int Hq, int G, int cols, bool two_heads,
+                      float scale_log2, int* status) {
   using C = PackedFwdCfg<D>;
   using T = Tile<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -145,16 +145,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int total_items = ld_global(counts + (two_heads ? 0 : 1)) * per_tile;
       bool ok = true;
       int ks = 0, kph = 0, vs = 0, vph = 0;  // ring positions
-      unsigned drawn = blockIdx.x;           // an item, or beyond total_items
+      int drawn = blockIdx.x;                // an item, or total_items or more: there is none
       const bool draws = total_items > static_cast<int>(gridDim.x);
       auto draw = [&]() {
-        if (lane == 0) drawn = draws ? atomicAdd(work_counter, 1u) : max(total_items, 1);
+        if (lane == 0) drawn = draws ? atomicAdd(counts + 2, 1) : total_items;
       };
       auto drawn_item = [&]() {  // the number drawn, for the whole warp
-        if (lane == 0) {
-          if (draws && drawn == total_items + gridDim.x - 1u) atomicExch(work_counter, 0u);
-          *next_slot = static_cast<int>(drawn);
-        }
+        if (lane == 0) *next_slot = drawn;
         __syncwarp();
         const int id = *next_slot;
         __syncwarp();
@@ -220,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (++vs == C::kStages) vs = 0, vph ^= 1;
           }
         }
-        if (!asked) draw();  // a CTA that gives up goes on drawing, once an item, so that the counter is left at zero
+        if (!asked) draw();
       }
     } else if (warp == 8) {
       // ---------------------------------------------------------------- S = Q_i K_j^T issuer
@@ -452,27 +449,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <int D, bool BF16, int KD = D>
 cudaError_t launch_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
-                     const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, const LaunchCtx& ctx, cudaStream_t stream) {
+                     const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms, cudaStream_t stream) {
   using C = PackedFwdCfg<D>;
   auto kern = packed_fwd_kernel<D, BF16, KD>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   const bool two_heads = s.Hq / s.Hkv % 2 == 0;
   const long long items = static_cast<long long>(plan.capacity) * (two_heads ? s.Hq / 2 : s.Hq);
-  const unsigned grid = static_cast<unsigned>(items < ctx.num_sms ? items : ctx.num_sms);
+  const unsigned grid = static_cast<unsigned>(items < num_sms ? items : num_sms);
   return launch_dependent(kern, grid, kThreads, C::kSmemBytes, stream, tq, tk, tv, to, static_cast<uint16_t*>(out), lse, plan.counts,
                           two_heads ? plan.tiles : plan.pairs, s.rows, s.Hq, s.Hq / s.Hkv, s.Dg, two_heads,
-                          s.scale * 1.4426950408889634f, ctx.status, ctx.work_counter);
+                          s.scale * 1.4426950408889634f, status);
 }
 
 }  // namespace
 
 cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
-                              const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, const LaunchCtx& ctx,
+                              const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms,
                               cudaStream_t stream) {
 #define FA2_CASE(DD, KK)                                                                          \
-  return s.dtype ? launch_t<DD, true, KK>(s, plan, tq, tk, tv, to, out, lse, ctx, stream)         \
-                 : launch_t<DD, false, KK>(s, plan, tq, tk, tv, to, out, lse, ctx, stream)
+  return s.dtype ? launch_t<DD, true, KK>(s, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)  \
+                 : launch_t<DD, false, KK>(s, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)
   if (s.D == 32) FA2_CASE(32, 32);
   if (s.D == 64) FA2_CASE(64, 64);
   if (s.Dg <= kShortDim128) FA2_CASE(128, kShortDim128);

@@ -268,7 +268,7 @@ int fa2_bwd_static_scratch(const void* q, const void* k, const void* v, const vo
  * word (0x80000), and every output is zero.
  * fa2_packed_fwd writes the order in which the kernels take the tiles of the sequences into `plan` (16-byte aligned,
  * fa2_packed_plan_bytes), which fa2_packed_bwd reads, and lse, fp32 [Hq, rows] (natural log; rows of no sequence are left
- * alone).  The work counter of fa2_fwd's note on captured calls is used here too: replays of one graph must not overlap.
+ * alone).
  * fa2_packed_bwd recomputes the scores for dK / dV and for dQ, so it needs no memory beyond O(rows): `workspace`
  * (16-byte aligned, fa2_packed_bwd_workspace_bytes) holds the row statistics.  dk and dv are summed over the query heads
  * of a key head in 32 bits; every sum has one owner and one order, so the same call gives the same bits.

@@ -206,6 +206,10 @@ def test_strided_inputs():
     heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in views]
     odd = [torch.nn.functional.pad(t, (0, 4))[..., :64] for t in views]  # rows 8 bytes apart from 16-byte boundaries
     assert torch.equal(run(*heads_first, cu_of(lengths))["o"], want["o"]) and torch.equal(run(*odd, cu_of(lengths))["o"], want["o"])
+    flat = torch.cat([fused.new_zeros(1), fused.flatten()])[1:]  # dense, 2 bytes behind a 16-byte boundary
+    odd = [flat.view(240, 8, 64)[:, a:b] for a, b in ((0, 4), (4, 6), (6, 8))]
+    assert torch.equal(run(*odd, cu_of(lengths))["o"], want["o"])
+    assert torch.equal(run(*odd, cu_of(lengths), torch.cat([do.new_zeros(1), do.contiguous().flatten()])[1:].view(240, 4, 64))["dk"], want["dk"])
     one = do[:, :1].expand(-1, 4, -1)  # a broadcast gradient
     a, b = run(*views, cu_of(lengths), one), run(*views, cu_of(lengths), one.contiguous())
     assert all(torch.equal(a[n], b[n]) for n in a)

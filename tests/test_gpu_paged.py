@@ -123,6 +123,7 @@ def test_append_strided_inputs():
     # rows that no kernel can read in place: a stride of 8 bytes more, columns apart
     odd = normal(50, 2, 68, dtype=BF16)[..., :64]
     wide = normal(50, 2, 128, dtype=BF16)[..., ::2]
+    odd = torch.cat([odd.new_zeros(1), odd.contiguous().flatten()])[1:].view(50, 2, 64)  # dense, 2 bytes behind a boundary
     fa.append_kv_cache(odd, wide, cache.k, cache.v, cache.table, cache.lengths([30, 20]), cu_seqlens=cu_seqlens_of([30, 20]))
     assert torch.equal(cache.k[cache.places(0, range(30))], odd[:30]) and torch.equal(cache.v[cache.places(1, range(20))], wide[30:])
 
