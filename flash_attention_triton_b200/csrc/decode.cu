@@ -34,14 +34,19 @@ constexpr int kWarps = 4;
 constexpr int kJoinRows = 8;  // query heads that the warps of a CTA add up at a time
 // Query heads of a key head that one pass takes: 8 for each column tile of the products.
 inline int column_tiles(int group) { return group <= 8 ? 1 : 2; }
+// Key heads that one pass takes.  Up to head dim 64 two: a warp's copies are twice as large then, and rows of 128 bytes that lie
+// beside each other are read at the same time.
+inline int heads_at_once(int Hkv, int D) { return D <= 64 && Hkv % 2 == 0 ? 2 : 1; }
 constexpr int kMaxCtas = 1024;
 
-template <int DP>
+template <int DP, int HP>
 struct DecodeCfg {
-  static constexpr int kStages = DP == 64 ? 4 : 3;
-  static constexpr int kCtasPerSm = DP == 64 ? 3 : (DP == 128 ? 2 : 1);
-  static constexpr int kChunks = DP / 64;           // of 64 columns, what a box of a copy is wide
-  static constexpr int kTileBytes = 16 * DP * 2;    // 16 keys, or 16 values: [kChunks][16 rows][128 bytes], swizzled
+  static_assert(HP == 1 || DP == 64, "two heads up to head dim 64");
+  static constexpr int kWide = DP * HP;             // columns of a stage's row
+  static constexpr int kStages = kWide == 64 ? 4 : 3;
+  static constexpr int kCtasPerSm = kWide == 64 ? 3 : (kWide == 128 ? 2 : 1);
+  static constexpr int kChunks = kWide / 64;        // of 64 columns, what a box of a copy is wide
+  static constexpr int kTileBytes = 16 * kWide * 2; // 16 keys, or 16 values: [kChunks][16 rows][128 bytes], swizzled
   static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
   static constexpr int kJoinStride = DP + 4;        // floats of a row of partial sums
   static constexpr int kOffJoin = kWarps * kWarpBytes;
@@ -51,9 +56,9 @@ struct DecodeCfg {
   static_assert(kCtasPerSm * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of one SM");
 };
 
-// One (sequence, key head) of the call, and the walk over the units of a CTA's stretch.
+// One (sequence, key head) of the call, or two key heads up to head dim 64 (HP), and the walk over the units of a CTA's stretch.
 struct Walk {
-  int b, h;
+  int b, h;    // the sequence; the number of the head, or pair of heads
   int unit;    // of it
   int units;   // of the sequence
   int length;  // keys of the sequence
@@ -69,39 +74,39 @@ __device__ __forceinline__ int units_of(int length) { return (length + kUnit - 1
 __device__ __forceinline__ int room_of(int length) { return length > 0 ? units_of(length) + kEnd : 0; }
 
 // Length of the row (whole warp).
-__device__ __forceinline__ long long row_length(const DecodeArgs& a, int lane) {
+__device__ __forceinline__ long long row_length(const DecodeArgs& a, int heads, int lane) {
   long long sum = 0;
   for (int i = 0; i < a.batch; i += 32) {
     const unsigned u = i + lane < a.batch ? room_of(clamp_length(a, i + lane)) : 0;
     sum += __reduce_add_sync(0xffffffffu, u);
   }
-  return sum * a.Hkv;
+  return sum * heads;
 }
 
 __device__ __forceinline__ long long stretch_start(long long total, int stretch, int stretches) { return total * stretch / stretches; }
 
-__device__ __forceinline__ void next_segment(const DecodeArgs& a, Walk& w) {
+__device__ __forceinline__ void next_segment(const DecodeArgs& a, int heads, Walk& w) {
   w.unit = 0;
-  if (++w.h < a.Hkv) return;
+  if (++w.h < heads) return;
   w.h = 0;
   do {
     w.length = ++w.b < a.batch ? clamp_length(a, w.b) : 1;
     w.units = units_of(w.length);
   } while (w.units == 0);
 }
-__device__ __forceinline__ void next_unit(const DecodeArgs& a, Walk& w) {
+__device__ __forceinline__ void next_unit(const DecodeArgs& a, int heads, Walk& w) {
   --w.left;
   if (++w.unit < w.units) return;
   w.left -= kEnd;
-  if (w.left > 0) next_segment(a, w);
+  if (w.left > 0) next_segment(a, heads, w);
 }
 
 // Puts `w` on the first unit of the stretch that begins at `at` of the row (whole warp); `at` is less than the row's length.
-__device__ __forceinline__ void find_unit(const DecodeArgs& a, long long at, int lane, Walk& w) {
+__device__ __forceinline__ void find_unit(const DecodeArgs& a, int heads, long long at, int lane, Walk& w) {
   for (int i = 0;; i += 32) {
     const int n = i + lane < a.batch ? clamp_length(a, i + lane) : 0;
     const unsigned mine = room_of(n);
-    const long long all = static_cast<long long>(__reduce_add_sync(0xffffffffu, mine)) * a.Hkv;
+    const long long all = static_cast<long long>(__reduce_add_sync(0xffffffffu, mine)) * heads;
     if (at >= all && i + 32 < a.batch) {
       at -= all;
       continue;
@@ -112,20 +117,20 @@ __device__ __forceinline__ void find_unit(const DecodeArgs& a, long long at, int
       const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    const unsigned in = __ballot_sync(0xffffffffu, static_cast<long long>(upto) * a.Hkv > at);
+    const unsigned in = __ballot_sync(0xffffffffu, static_cast<long long>(upto) * heads > at);
     const int l = __ffs(in) - 1;
     const int room = __shfl_sync(0xffffffffu, mine, l);
     w.b = i + l;
     w.units = room - kEnd;
     w.length = __shfl_sync(0xffffffffu, n, l);
-    const int rest = static_cast<int>(at - static_cast<long long>(__shfl_sync(0xffffffffu, upto - mine, l)) * a.Hkv);
+    const int rest = static_cast<int>(at - static_cast<long long>(__shfl_sync(0xffffffffu, upto - mine, l)) * heads);
     w.h = rest / room;
     w.unit = rest - w.h * room;
     break;
   }
   if (w.unit >= w.units) {  // in the room behind the units
     w.left -= w.units + kEnd - w.unit;
-    if (w.left > 0) next_segment(a, w);
+    if (w.left > 0) next_segment(a, heads, w);
   }
 }
 
@@ -182,12 +187,12 @@ struct Workspace {
   __device__ float* part(int place, int rows, int D) const { return parts + static_cast<long long>(place) * rows * (D + 2); }
 };
 
-template <int DP, int NT, bool BF16>
-__global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
+template <int DP, int HP, int NT, bool BF16>
+__global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ DecodeArgs a, int rows, int slots, int box_rows, int* status) {
-  using C = DecodeCfg<DP>;
-  constexpr int kRows = 8 * NT;
+  using C = DecodeCfg<DP, HP>;
+  constexpr int kRows = 8 * NT, kSteps = DP / 16;  // columns of a head in sixteens
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = smem_u32(smem);
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   const WaitCtx w{abort_flag, status};
   const int group = a.Hq / a.Hkv, blocks = (group + kRows - 1) / kRows;
   const int stretches = gridDim.x / blocks, stretch = blockIdx.x / blocks, pass = blockIdx.x - stretch * blocks;
-  const int d8 = a.D / 8;
+  const int heads = a.Hkv / HP, d8 = a.D / 8;
 
   if (lane == 0)
     for (int s = 0; s < C::kStages; ++s) mbar_init(bar(s), 1);
@@ -219,20 +224,20 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   grid_allow_next();
 
   const Workspace space(a.workspace, slots, gridDim.x);
-  const bool by_segment = static_cast<long long>(a.batch) * a.Hkv * blocks == slots;  // what a Cut belongs to
+  const bool by_segment = static_cast<long long>(a.batch) * heads * blocks == slots;  // what a Cut belongs to
   // sequences without keys
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
     if (ld_global(a.lengths + b) <= 0) {
       for (int i = threadIdx.x; i < a.Hq * d8; i += 32 * kWarps)
         reinterpret_cast<uint4*>(a.out)[static_cast<long long>(b) * a.Hq * d8 + i] = make_uint4(0, 0, 0, 0);
       if (by_segment)
-        for (int h = threadIdx.x; h < a.Hkv * blocks; h += 32 * kWarps) space.cuts[b * a.Hkv * blocks + h] = make_int4(0, 0, 0, -1);
+        for (int h = threadIdx.x; h < heads * blocks; h += 32 * kWarps) space.cuts[b * heads * blocks + h] = make_int4(0, 0, 0, -1);
     }
 
-  const long long total = row_length(a, lane);
+  const long long total = row_length(a, heads, lane);
   const long long u0 = stretch_start(total, stretch, stretches), u1 = stretch_start(total, stretch + 1, stretches);
   Walk load{0, 0, 0, 0, 0, static_cast<int>(u1 - u0)};
-  if (load.left > 0) find_unit(a, u0, lane, load);
+  if (load.left > 0) find_unit(a, heads, u0, lane, load);
   if (threadIdx.x == 0) space.counts[blockIdx.x] = load.left > 0;
   if (load.left <= 0) {
     if (!by_segment && threadIdx.x == 0) space.cuts[blockIdx.x] = make_int4(0, 0, 0, -1);
@@ -265,19 +270,20 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     keys = __reduce_or_sync(0xffffffffu, keys);
     if (copies != 0) {
       const uint32_t dst = ring + stage * 2 * C::kTileBytes;
-      if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * DP * 4);
+      if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * C::kWide * 4);
       __syncwarp();
       if (take) {
-        const int kv_head = load.h;
 #pragma unroll
         for (int ch = 0; ch < C::kChunks; ++ch) {
           const uint32_t to = dst + ch * 2048 + lane * box_rows * 128;
-          tma_load_4d(to, &tk, ch * 64, slot, HeadCoord{kv_head, page}, bar(stage));
-          tma_load_4d(to + C::kTileBytes, &tv, ch * 64, slot, HeadCoord{kv_head, page}, bar(stage));
+          const int x = HP == 2 ? 0 : ch * 64;
+          const HeadCoord from{HP == 2 ? 2 * load.h + ch : load.h, page};
+          tma_load_4d(to, &tk, x, slot, from, bar(stage));
+          tma_load_4d(to + C::kTileBytes, &tv, x, slot, from, bar(stage));
         }
       }
     }
-    next_unit(a, load);
+    next_unit(a, heads, load);
     if (load.left > 0) look_up();
     return keys;
   };
@@ -286,9 +292,9 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
 #pragma unroll
   for (int s = 0; s < C::kStages; ++s) valid[s] = load.left > 0 ? issue(s) : 0u;
 
-  uint32_t qb[DP / 16][NT][2];
-  float o[DP / 16][NT][4];  // rows (columns of V) 16 i + lane / 4 (+ 8), columns (query heads) 8 t + 2 (lane % 4) (+ 1)
-  float m[NT][2], l[NT][2];
+  uint32_t qb[HP][kSteps][NT][2];
+  float o[HP][kSteps][NT][4];  // rows (columns of V) 16 i + lane / 4 (+ 8), columns (query heads) 8 t + 2 (lane % 4) (+ 1)
+  float m[HP][NT][2], l[HP][NT][2];
   const float threshold = 8.f / a.scale_log2;
   uint32_t phases = 0;  // bit s: parity of the next wait on stage s
   bool fresh = true, ok = true;
@@ -296,27 +302,33 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
   int stage = 0;
   const int here = min(kRows, group - pass * kRows);  // query heads in use
   auto load_q = [&]() {
-    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + work.b * a.sq.row + (work.h * group + pass * kRows) * a.sq.head;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int p = 0; p < HP; ++p) {
+      const uint16_t* const q =
+          static_cast<const uint16_t*>(a.q) + work.b * a.sq.row + ((work.h * HP + p) * group + pass * kRows) * a.sq.head;
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int head = 8 * t + lane / 4, col = 16 * i + 8 * j + (lane & 3) * 2;
-          qb[i][t][j] = head < here && col < a.D ? ld_global(reinterpret_cast<const unsigned*>(q + head * a.sq.head + col)) : 0u;
-        }
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int head = 8 * t + lane / 4, col = 16 * i + 8 * j + (lane & 3) * 2;
+            qb[p][i][t][j] = head < here && col < a.D ? ld_global(reinterpret_cast<const unsigned*>(q + head * a.sq.head + col)) : 0u;
+          }
+    }
   };
   load_q();
   while (work.left > 0) {
     if (fresh) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
+      for (int p = 0; p < HP; ++p)
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
-      }
+        for (int t = 0; t < NT; ++t) {
+          m[p][t][0] = m[p][t][1] = -INFINITY;
+          l[p][t][0] = l[p][t][1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) o[p][i][t][0] = o[p][i][t][1] = o[p][i][t][2] = o[p][i][t][3] = 0.f;
+        }
     }
     // ---- one unit: this warp's 16 keys
     const uint32_t mine = valid[0];
@@ -333,79 +345,87 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
       }
       // row of this lane in the 16 x 16 piece of a tile that ldmatrix takes, and which half of its columns
       const int krow = (lane & 7) + (lane & 8), khalf = lane >> 4;
-      float s[NT][4] = {};
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        uint32_t x[4];
-        load_matrices(ktile + (k / 4) * 2048 + krow * 128 + (((2 * (k % 4) + khalf) ^ (krow & 7)) << 4), x);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) product<BF16>(s[t], x, qb[k][t][0], qb[k][t][1]);
-      }
       const bool in0 = (mine >> (lane / 4)) & 1u, in1 = (mine >> (lane / 4 + 8)) & 1u;
+      float s[HP][NT][4] = {};
       bool need = false;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int p = 0; p < HP; ++p) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (!in0) s[t][e] = -INFINITY;
-          if (!in1) s[t][2 + e] = -INFINITY;
-          need |= fmaxf(s[t][e], s[t][2 + e]) - m[t][e] > threshold;
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t x[4];
+          load_matrices(ktile + ((p * kSteps + k) / 4) * 2048 + krow * 128 + (((2 * (k % 4) + khalf) ^ (krow & 7)) << 4), x);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) product<BF16>(s[p][t], x, qb[p][k][t][0], qb[p][k][t][1]);
         }
-      // The maximum follows only when a score is 2^8 above it: a weight is at most 2^8 then.
-      if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[t][e], s[t][2 + e]);
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            x = fmaxf(x, m[t][e]);
-            // a head without a finite score so far has weights 0
-            const float alpha = x == -INFINITY ? 1.f : ex2((m[t][e] - x) * a.scale_log2);
-            m[t][e] = x;
-            l[t][e] *= alpha;
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) o[i][t][e] *= alpha, o[i][t][2 + e] *= alpha;
+            if (!in0) s[p][t][e] = -INFINITY;
+            if (!in1) s[p][t][2 + e] = -INFINITY;
+            need |= fmaxf(s[p][t][e], s[p][t][2 + e]) - m[p][t][e] > threshold;
           }
+      }
+      // The maximum follows only when a score is 2^8 above it: a weight is at most 2^8 then.
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int p = 0; p < HP; ++p)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(s[p][t][e], s[p][t][2 + e]);
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              x = fmaxf(x, m[p][t][e]);
+              // a head without a finite score so far has weights 0
+              const float alpha = x == -INFINITY ? 1.f : ex2((m[p][t][e] - x) * a.scale_log2);
+              m[p][t][e] = x;
+              l[p][t][e] *= alpha;
+#pragma unroll
+              for (int i = 0; i < kSteps; ++i) o[p][i][t][e] *= alpha, o[p][i][t][2 + e] *= alpha;
+            }
       }
       // P^T in 16 bits; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
       // term is p (1 - 2^-8) rounded, at most p (1 - 2^-16), so that the second one is positive where p is, and an
       // infinite value stays infinite in both products.
-      uint32_t p[NT][2], rest[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float shift = m[t][e] == -INFINITY ? 0.f : -m[t][e] * a.scale_log2;
-          s[t][e] = ex2(fmaf(s[t][e], a.scale_log2, shift));
-          s[t][2 + e] = ex2(fmaf(s[t][2 + e], a.scale_log2, shift));
-          l[t][e] += s[t][e] + s[t][2 + e];
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float x = s[t][2 * j], y = s[t][2 * j + 1];
-          if constexpr (BF16) {
-            const uint32_t both = pack2<BF16>(x * 0.99609375f, y * 0.99609375f);
-            const float2 f = unpack2<BF16>(both);
-            p[t][j] = turned(both);
-            rest[t][j] = turned(pack2<BF16>(x - f.x, y - f.y));
-          } else {
-            p[t][j] = turned(pack2<BF16>(x, y));
-          }
-        }
-      }
-      // V^T: the 16 x 16 piece of V is turned around on its way, so the lanes' rows and halves change places
+      // V^T: the 16 x 16 piece of V is turned around on its way, so the lanes' rows and halves change places.
       const int vrow = (lane & 7) + ((lane >> 4) << 3), vhalf = (lane >> 3) & 1;
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        uint32_t x[4];
-        load_matrices_t(vtile + (i / 4) * 2048 + vrow * 128 + (((2 * (i % 4) + vhalf) ^ (vrow & 7)) << 4), x);
+      for (int p = 0; p < HP; ++p) {
+        uint32_t weight[NT][2], rest[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          product<BF16>(o[i][t], x, p[t][0], p[t][1]);
-          if constexpr (BF16) product<BF16>(o[i][t], x, rest[t][0], rest[t][1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float shift = m[p][t][e] == -INFINITY ? 0.f : -m[p][t][e] * a.scale_log2;
+            s[p][t][e] = ex2(fmaf(s[p][t][e], a.scale_log2, shift));
+            s[p][t][2 + e] = ex2(fmaf(s[p][t][2 + e], a.scale_log2, shift));
+            l[p][t][e] += s[p][t][e] + s[p][t][2 + e];
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float x = s[p][t][2 * j], y = s[p][t][2 * j + 1];
+            if constexpr (BF16) {
+              const uint32_t both = pack2<BF16>(x * 0.99609375f, y * 0.99609375f);
+              const float2 f = unpack2<BF16>(both);
+              weight[t][j] = turned(both);
+              rest[t][j] = turned(pack2<BF16>(x - f.x, y - f.y));
+            } else {
+              weight[t][j] = turned(pack2<BF16>(x, y));
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          uint32_t x[4];
+          load_matrices_t(vtile + ((p * kSteps + i) / 4) * 2048 + vrow * 128 + (((2 * (i % 4) + vhalf) ^ (vrow & 7)) << 4), x);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            product<BF16>(o[p][i][t], x, weight[t][0], weight[t][1]);
+            if constexpr (BF16) product<BF16>(o[p][i][t], x, rest[t][0], rest[t][1]);
+          }
         }
       }
     }
@@ -420,35 +440,36 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
     // next queries on their way
     const Walk now = work;
     const bool ends = now.unit + 1 == now.units;
-    next_unit(a, work);
+    next_unit(a, heads, work);
     fresh = ends || work.left <= 0;
     if (fresh) {
       if (work.left > 0) load_q();
       const bool whole = begins && ends;
-      const int head0 = now.h * group + pass * kRows;
-      float* const part = space.part(2 * blockIdx.x + (begins ? 1 : 0), rows, a.D);
+      float* const part = space.part(2 * blockIdx.x + (begins ? 1 : 0), HP * rows, a.D);
       if (threadIdx.x == 0 && (by_segment ? begins : work.left <= 0)) {
         // the stretch of a unit is the last one that starts at or before it
         const long long last = u1 - now.left + (now.units - 1 - now.unit);
         const int end = begins && !ends ? static_cast<int>(((last + 1) * stretches - 1) / total) : -1;
-        space.cuts[by_segment ? (now.b * a.Hkv + now.h) * blocks + pass : blockIdx.x] = make_int4(now.b, now.h, stretch, end);
+        space.cuts[by_segment ? (now.b * heads + now.h) * blocks + pass : blockIdx.x] = make_int4(now.b, now.h, stretch, end);
       }
       begins = true;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int pt = 0; pt < HP * NT; ++pt) {
+        const int p = pt / NT, t = pt % NT;
         const int row0 = t * kJoinRows, some = min(here - row0, kJoinRows);
-        if (some <= 0) break;
+        if (some <= 0) continue;
+        const int head0 = (now.h * HP + p) * group + pass * kRows + row0;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float sum = l[t][e];
+          float sum = l[p][t][e];
           sum += __shfl_xor_sync(0xffffffffu, sum, 4);
           sum += __shfl_xor_sync(0xffffffffu, sum, 8);
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           const int row = warp * kJoinRows + (lane & 3) * 2 + e;
           float* const to = join + row * C::kJoinStride + lane / 4;
 #pragma unroll
-          for (int i = 0; i < DP / 16; ++i) to[16 * i] = o[i][t][e], to[16 * i + 8] = o[i][t][2 + e];
-          if (lane < 4) *reinterpret_cast<float2*>(join_ml + row * 2) = make_float2(m[t][e], sum);
+          for (int i = 0; i < kSteps; ++i) to[16 * i] = o[p][i][t][e], to[16 * i + 8] = o[p][i][t][2 + e];
+          if (lane < 4) *reinterpret_cast<float2*>(join_ml + row * 2) = make_float2(m[p][t][e], sum);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < some * (a.D / 2); i += 32 * kWarps) {
@@ -469,11 +490,12 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
           }
           if (whole) {
             const float inv = 1.f / all;
-            uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(now.b) * a.Hq + head0 + row0 + row) * a.D + col;
+            uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(now.b) * a.Hq + head0 + row) * a.D + col;
             *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(sum.x * inv, sum.y * inv);
           } else {
-            *reinterpret_cast<float2*>(part + 2 * rows + (row0 + row) * a.D + col) = sum;
-            if (col == 0) *reinterpret_cast<float2*>(part + 2 * (row0 + row)) = make_float2(top, all);
+            const int r = p * rows + row0 + row;  // of the place
+            *reinterpret_cast<float2*>(part + 2 * HP * rows + r * a.D + col) = sum;
+            if (col == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(top, all);
           }
         }
         __syncthreads();
@@ -488,22 +510,23 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP>::kCtasPerSm)
 constexpr int kJoinThreads = 256;
 template <bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass_heads,
-                                                                   int slots, int ctas) {
+                                                                   int hp, int slots, int ctas) {
   __shared__ float weight[kJoinThreads], reduced[kJoinThreads / 32];
   __shared__ float2 sums[kJoinThreads];
   grid_wait_previous();
   grid_allow_next();
   const Workspace space(a.workspace, slots, ctas);
-  const uint4 c = ld_global(reinterpret_cast<const uint4*>(space.cuts) + blockIdx.x / rows);
+  const int place_rows = hp * rows;
+  const uint4 c = ld_global(reinterpret_cast<const uint4*>(space.cuts) + blockIdx.x / place_rows);
   const Cut cut{static_cast<int>(c.x), static_cast<int>(c.y), static_cast<int>(c.z), static_cast<int>(c.w)};
-  const int row = blockIdx.x % rows;
-  const int group = a.Hq / a.Hkv, blocks = (group + pass_heads - 1) / pass_heads, pass = blockIdx.x / rows % blocks;
-  const int in_group = pass * pass_heads + row;
+  const int row = blockIdx.x % place_rows;
+  const int group = a.Hq / a.Hkv, blocks = (group + pass_heads - 1) / pass_heads, pass = blockIdx.x / place_rows % blocks;
+  const int in_group = pass * pass_heads + row % rows;
   if (cut.last < 0 || in_group >= group) return;
   const int parts = cut.last - cut.first + 1, d2 = a.D / 2;
   const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = kJoinThreads / d2;
   auto cta = [&](int i) { return (cut.first + i) * blocks + pass; };
-  auto part = [&](int i) { return space.part(2 * cta(i) + (i == 0 ? 1 : 0), rows, a.D); };
+  auto part = [&](int i) { return space.part(2 * cta(i) + (i == 0 ? 1 : 0), place_rows, a.D); };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top = -INFINITY, all = 0.f;
   float2 sum = make_float2(0.f, 0.f);
@@ -540,7 +563,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
 #pragma unroll 8
       for (int i = share; i < here; i += shares) {
         const float f = weight[i];
-        const float2 x = ld_global(reinterpret_cast<const float2*>(part(p0 + i) + 2 * rows + row * a.D + 2 * col));
+        const float2 x = ld_global(reinterpret_cast<const float2*>(part(p0 + i) + 2 * place_rows + row * a.D + 2 * col));
         // (weight 0: the part may have been left out, and hold anything)
         sum.x = f == 0.f ? sum.x : fmaf(f, x.x, sum.x);
         sum.y = f == 0.f ? sum.y : fmaf(f, x.y, sum.y);
@@ -555,31 +578,31 @@ __global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_
       sum.x += x.x, sum.y += x.y;
     }
     const float inv = 1.f / all;  // NaN for a row without any finite score, as everywhere
-    uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.b) * a.Hq + cut.h * group + in_group) * a.D + 2 * col;
+    uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.b) * a.Hq + (cut.h * hp + row / rows) * group + in_group) * a.D + 2 * col;
     *reinterpret_cast<uint32_t*>(to) = pack2<BF16>(sum.x * inv, sum.y * inv);
   }
 }
 
 // CTAs of decode_kernel, of `slots` that run at a time: a multiple of the passes, no more than units of the call.
 struct DecodeGrid {
-  int rows, passes, ctas, cuts;
+  int hp, rows, ctas, cuts;  // key heads and query heads that a pass takes; CTAs; Cuts
 };
-DecodeGrid decode_grid(int batch, int Hq, int Hkv, int table_width, int page_size, int slots) {
-  const int group = Hq / Hkv, take = 8 * column_tiles(group), passes = (group + take - 1) / take;
-  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit * batch * Hkv;
-  const long long stretches = std::max(1, slots / passes), segments = static_cast<long long>(batch) * Hkv * passes;
+DecodeGrid decode_grid(int batch, int Hq, int Hkv, int D, int table_width, int page_size, int slots) {
+  const int hp = heads_at_once(Hkv, D), group = Hq / Hkv, take = 8 * column_tiles(group), passes = (group + take - 1) / take;
+  const long long units = (static_cast<long long>(table_width) * page_size + kUnit - 1) / kUnit * batch * (Hkv / hp);
+  const long long stretches = std::max(1, slots / passes), segments = static_cast<long long>(batch) * (Hkv / hp) * passes;
   const int ctas = static_cast<int>(std::min(units, stretches) * passes);
-  return DecodeGrid{std::min(group, take), passes, ctas, static_cast<int>(std::min<long long>(segments, ctas))};
+  return DecodeGrid{hp, std::min(group, take), ctas, static_cast<int>(std::min<long long>(segments, ctas))};
 }
 
-template <int DP, int NT, bool BF16>
+template <int DP, int HP, int NT, bool BF16>
 cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int box_rows, int num_sms, int* status,
                             cudaStream_t stream) {
-  using C = DecodeCfg<DP>;
-  auto kern = decode_kernel<DP, NT, BF16>;
+  using C = DecodeCfg<DP, HP>;
+  auto kern = decode_kernel<DP, HP, NT, BF16>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
-  const DecodeGrid g = decode_grid(a.batch, a.Hq, a.Hkv, a.table_width, a.page_size, std::min(num_sms * C::kCtasPerSm, kMaxCtas));
+  const DecodeGrid g = decode_grid(a.batch, a.Hq, a.Hkv, a.D, a.table_width, a.page_size, std::min(num_sms * C::kCtasPerSm, kMaxCtas));
   // With more than one CTA to an SM an ordinary launch.  CTAs that start under the end of the kernel before find small blocks
   // of shared memory taken in the middle of an SM's and settle around them; what these leave behind is in two pieces, too small
   // for the SM's last CTA, which then runs after the others (64 sequences of 204 000 keys, 12 heads of 64 columns:
@@ -591,16 +614,16 @@ cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const 
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;
-  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows, kJoinThreads, 0, stream, a, g.rows, 8 * NT, g.cuts,
-                          g.ctas);
+  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows * HP, kJoinThreads, 0, stream, a, g.rows, 8 * NT, HP,
+                          g.cuts, g.ctas);
 }
 
 }  // namespace
 
 size_t decode_workspace_floats(int batch, int Hq, int Hkv, int D, int table_width, int page_size) {
   // (more CTAs than this never run; the largest number of passes may need more)
-  const DecodeGrid g = decode_grid(batch, Hq, Hkv, table_width, page_size, kMaxCtas);
-  return static_cast<size_t>(Workspace::floats(g.cuts, g.ctas, g.rows, D));
+  const DecodeGrid g = decode_grid(batch, Hq, Hkv, D, table_width, page_size, kMaxCtas);
+  return static_cast<size_t>(Workspace::floats(g.cuts, g.ctas, g.hp * g.rows, D));
 }
 
 int decode_box_rows(int page_size) {
@@ -612,15 +635,16 @@ int decode_box_rows(int page_size) {
 cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int dtype, int num_sms, int* status,
                           cudaStream_t stream) {
   const int box = decode_box_rows(a.page_size), tiles = column_tiles(a.Hq / a.Hkv);
-#define FA2_CASE(DP)                                                                                         \
+#define FA2_CASE(DP, HP)                                                                                     \
   if (tiles == 1)                                                                                            \
-    return dtype ? launch_decode_t<DP, 1, true>(tk, tv, a, box, num_sms, status, stream)                     \
-                 : launch_decode_t<DP, 1, false>(tk, tv, a, box, num_sms, status, stream);                   \
-  return dtype ? launch_decode_t<DP, 2, true>(tk, tv, a, box, num_sms, status, stream)                       \
-               : launch_decode_t<DP, 2, false>(tk, tv, a, box, num_sms, status, stream)
-  if (a.D <= 64) { FA2_CASE(64); }
-  if (a.D <= 128) { FA2_CASE(128); }
-  FA2_CASE(256);
+    return dtype ? launch_decode_t<DP, HP, 1, true>(tk, tv, a, box, num_sms, status, stream)                 \
+                 : launch_decode_t<DP, HP, 1, false>(tk, tv, a, box, num_sms, status, stream);               \
+  return dtype ? launch_decode_t<DP, HP, 2, true>(tk, tv, a, box, num_sms, status, stream)                   \
+               : launch_decode_t<DP, HP, 2, false>(tk, tv, a, box, num_sms, status, stream)
+  if (a.D <= 64 && heads_at_once(a.Hkv, a.D) == 2) { FA2_CASE(64, 2); }
+  if (a.D <= 64) { FA2_CASE(64, 1); }
+  if (a.D <= 128) { FA2_CASE(128, 1); }
+  FA2_CASE(256, 1);
 #undef FA2_CASE
 }
 

@@ -92,8 +92,9 @@ def test_workspace_size():
     lib = _lib.lib()
     # 16 bytes for every (sequence, key head) or CTA, whichever are fewer, 4 for every CTA (in fours), and two places for each
     # CTA: m, l and o of each row; no more CTAs than units of 64 keys
-    assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 16, 4) == 2 * 16 + 4 * 4 + 2 * 2 * 4 * 66 * 4
-    assert lib.fa2_decode_workspace_bytes(1, 40, 2, 64, 16, 8) == 4 * 16 + 8 * 4 + 8 * 2 * 16 * 66 * 4  # 20 heads: two passes of 16 rows
+    assert lib.fa2_decode_workspace_bytes(1, 8, 2, 128, 16, 4) == 2 * 16 + 4 * 4 + 2 * 2 * 4 * 130 * 4
+    assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 16, 4) == 1 * 16 + 4 * 4 + 1 * 2 * (2 * 4) * 66 * 4  # two key heads at once
+    assert lib.fa2_decode_workspace_bytes(1, 40, 2, 128, 16, 8) == 4 * 16 + 8 * 4 + 8 * 2 * 16 * 130 * 4  # 20 heads: two passes of 16 rows
     assert lib.fa2_decode_workspace_bytes(1, 3, 2, 64, 16, 4) == 0
     assert lib.fa2_decode_workspace_bytes(1, 8, 2, 64, 1 << 16, 1 << 16) == 0
 
