@@ -24,19 +24,25 @@ at::Tensor bytes_on(const at::Tensor& t, size_t n) {
 }
 cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// The plan and, behind it, lse in one allocation.
+size_t lse_offset(const Sizes& n) { return fa2_packed_plan_bytes(n.rows, n.batch); }
+size_t scratch_bytes(const Sizes& n) { return lse_offset(n) + 4ull * n.Hq * n.rows; }
+float* lse_of(const at::Tensor& scratch, const Sizes& n) {
+  return reinterpret_cast<float*>(static_cast<char*>(scratch.data_ptr()) + lse_offset(n));
+}
+
 struct Forward {
-  at::Tensor out, lse, plan;
+  at::Tensor out, scratch;
 };
 // q, k and v are replaced by what the kernels read.
 Forward run_forward(at::Tensor& q, at::Tensor& k, at::Tensor& v, const at::Tensor& cu, const Sizes& n, double scale) {
   const c10::cuda::CUDAGuard guard(q.device());
   q = rows_input(q), k = rows_input(k), v = rows_input(v);
-  Forward r{dense_like(q), at::empty({n.Hq, n.rows}, q.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous)),
-            bytes_on(q, fa2_packed_plan_bytes(n.rows, n.batch))};
+  Forward r{dense_like(q), bytes_on(q, scratch_bytes(n))};
   if (n.rows == 0) return r;
   const auto strides = strides_of<3>({&q, &k, &v});
-  check_code("fa2_packed_fwd", fa2_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.out.data_ptr(), r.lse.data_ptr<float>(),
-                                              cu.data_ptr<int>(), r.plan.data_ptr(), n.rows, n.batch, n.Hq, n.Hkv, n.D, dtype_code(q),
+  check_code("fa2_packed_fwd", fa2_packed_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), r.out.data_ptr(), lse_of(r.scratch, n),
+                                              cu.data_ptr<int>(), r.scratch.data_ptr(), n.rows, n.batch, n.Hq, n.Hkv, n.D, dtype_code(q),
                                               static_cast<float>(scale), strides.data(), stream_of(q)));
   return r;
 }
@@ -45,7 +51,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   // `r` holds the outputs of the forward kernel, already launched on saved q, k and v.
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                             const std::array<at::Tensor, 3>& saved, const at::Tensor& cu, const Forward& r, double scale) {
-    ctx->save_for_backward({saved[0], saved[1], saved[2], cu, r.out, r.lse, r.plan});
+    ctx->save_for_backward({saved[0], saved[1], saved[2], cu, r.out, r.scratch});
     ctx->saved_data["scale"] = scale;
     return r.out.view(r.out.sizes());  // the tensor that is saved is not the one handed out
   }
@@ -53,22 +59,22 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), "flash_attention_packed has no second derivative: do not pass create_graph=True");
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &cu = saved[3], &out = saved[4], &lse = saved[5], &plan = saved[6];
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &cu = saved[3], &out = saved[4], &scratch = saved[5];
     // saved-tensor hooks must give back what was saved
     TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && out.sizes() == q.sizes() && k.size(0) == q.size(0) &&
-                    k.size(2) == q.size(2) && lse.dim() == 2 && lse.size(0) == q.size(1) && lse.size(1) == q.size(0) && cu.dim() == 1 &&
-                    cu.size(0) > 1 && plan.nbytes() >= fa2_packed_plan_bytes(q.size(0), cu.size(0) - 1) && q.size(1) % k.size(1) == 0,
+                    k.size(2) == q.size(2) && cu.dim() == 1 && cu.size(0) > 1 && k.size(1) > 0 && q.size(1) % k.size(1) == 0,
                 "the saved tensors have changed their shapes");
     for (const at::Tensor* t : {&q, &k, &v, &out})
       TORCH_CHECK(is_16bit(*t) && t->scalar_type() == q.scalar_type() && rows_readable(*t), "the saved tensors have changed their type or strides");
-    TORCH_CHECK(out.is_contiguous() && lse.is_contiguous() && lse.scalar_type() == at::kFloat && cu.is_contiguous() &&
-                    cu.scalar_type() == at::kInt && plan.is_contiguous(), "the saved tensors have changed their type or strides");
-    at::Tensor dout = grads[0];
-    TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of the output");
-    for (const at::Tensor* t : {&q, &k, &v, &cu, &out, &lse, &plan, static_cast<const at::Tensor*>(&dout)})
-      TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "the saved tensors or the gradient are on another device");
     const Sizes n{static_cast<int>(q.size(0)), static_cast<int>(cu.size(0)) - 1, static_cast<int>(q.size(1)), static_cast<int>(k.size(1)),
                   static_cast<int>(q.size(2))};
+    TORCH_CHECK(out.is_contiguous() && cu.is_contiguous() && cu.scalar_type() == at::kInt && scratch.is_contiguous() &&
+                    scratch.nbytes() == scratch_bytes(n) && reinterpret_cast<uintptr_t>(scratch.data_ptr()) % 16 == 0,
+                "the saved tensors have changed their type or strides");
+    at::Tensor dout = grads[0];
+    TORCH_CHECK(dout.sizes() == q.sizes(), "the gradient must have the shape of the output");
+    for (const at::Tensor* t : {&q, &k, &v, &cu, &out, &scratch, static_cast<const at::Tensor*>(&dout)})
+      TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "the saved tensors or the gradient are on another device");
     const c10::cuda::CUDAGuard guard(q.device());
     if (dout.scalar_type() != q.scalar_type()) dout = dout.to(q.scalar_type());
     dout = rows_input(dout.is_neg() ? dout.resolve_neg() : dout);
@@ -78,8 +84,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       const at::Tensor workspace = bytes_on(q, bytes);
       const auto strides = strides_of<4>({&q, &k, &v, &dout});
       check_code("fa2_packed_bwd",
-                 fa2_packed_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(),
-                                dk.data_ptr(), dv.data_ptr(), cu.data_ptr<int>(), plan.data_ptr(), workspace.data_ptr(), bytes, n.rows,
+                 fa2_packed_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse_of(scratch, n), dq.data_ptr(),
+                                dk.data_ptr(), dv.data_ptr(), cu.data_ptr<int>(), scratch.data_ptr(), workspace.data_ptr(), bytes, n.rows,
                                 n.batch, n.Hq, n.Hkv, n.D, dtype_code(q), static_cast<float>(ctx->saved_data["scale"].toDouble()),
                                 strides.data(), stream_of(q)));
     }

@@ -330,3 +330,23 @@ def test_on_the_other_device():
     want = run(q, k, v, cu_of([100, 30]), do)
     got = run(*(t.to("cuda:1") for t in (q, k, v)), cu_of([100, 30]).to("cuda:1"), do.to("cuda:1"))
     assert all(torch.equal(got[n].cpu(), want[n].cpu()) for n in want)
+
+
+def test_saved_tensor_hooks():
+    """Saved tensors may leave the GPU and come back; one that comes back changed is refused."""
+    lengths = [90, 40]
+    q, k, v, do = inputs(lengths, 4, 2, 64, BF16)
+    want = run(q, k, v, cu_of(lengths), do)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    with torch.autograd.graph.save_on_cpu():
+        o = flash_attention_packed(*leaves, cu_of(lengths))
+    assert all(torch.equal(a, want[n]) for n, a in zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        o = flash_attention_packed(*leaves, cu_of(lengths))
+    with pytest.raises(RuntimeError, match="have changed"):
+        torch.autograd.grad(o, leaves, do)
+    o = flash_attention_packed(*leaves, cu_of(lengths))
+    with torch.no_grad():
+        k.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o, leaves, do)
