@@ -69,8 +69,9 @@ int fa2_packed_fwd(const void* q, const void* k, const void* v, void* o, float* 
   const PackedShape s = make_shape(rows, batch, Hq, Hkv, D, dtype, scale);
   const PackedPlan p = packed_plan(plan, rows, batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cudaError_t e = launch_packed_plan(s, cu_seqlens, p, Hq / Hkv % 2 != 0, o, ctx.status, ctx.num_sms, st)) return static_cast<int>(e);
-  return static_cast<int>(launch_packed_fwd(s, p, tq, tk, tv, to, o, lse, ctx.status, ctx.num_sms, st));
+  if (!packed_fwd_alone(s, ctx.num_sms))
+    if (cudaError_t e = launch_packed_plan(s, cu_seqlens, p, Hq / Hkv % 2 != 0, o, ctx.status, ctx.num_sms, st)) return static_cast<int>(e);
+  return static_cast<int>(launch_packed_fwd(s, cu_seqlens, p, tq, tk, tv, to, o, lse, ctx.status, ctx.num_sms, st));
 }
 
 size_t fa2_packed_bwd_workspace_bytes(int rows, int batch, int Hq) {

@@ -88,36 +88,6 @@ __device__ int write_list(const int* cu_seqlens, int batch, int per, PackedTile*
   return all;
 }
 
-// The same for up to 32 sequences, one a lane: entry t of a sequence comes behind those of higher numbers in all sequences and
-// those of the same number in the sequences before it, which a warp counts without a word to the others.
-__device__ __forceinline__ int write_short_list(int start, int length, int per, PackedTile* list) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int tiles = (length + 127) >> 7, n = (tiles + per - 1) / per;
-  int base = tiles;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, base, o);
-    if (lane >= o) base += y;
-  }
-  base -= tiles;
-  const int most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n));
-  for (int t = warp; t < most; t += warps) {
-    const int higher = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - t - 1, 0)));
-    const unsigned same = __ballot_sync(0xffffffffu, n > t);
-    if (n > t)
-      *reinterpret_cast<int4*>(list + higher + __popc(same & ((1u << lane) - 1u))) = make_int4(start, length, t * per, base);
-  }
-  return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
-}
-
-// Zeros in the rows of a dense [rows, row16 * 8] tensor that no sequence has.
-__device__ void clear_outside(void* out, long long row16, int first, int last, int rows, long long worker, long long workers) {
-  if (out == nullptr) return;
-  uint4* const p = static_cast<uint4*>(out);
-  for (long long i = worker; i < first * row16; i += workers) p[i] = make_uint4(0, 0, 0, 0);
-  for (long long i = last * row16 + worker; i < rows * row16; i += workers) p[i] = make_uint4(0, 0, 0, 0);
-}
-
 // CTA 0 writes the plan, the others clear the rows of `out` that no sequence has.
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu_seqlens, PackedPlan plan, int batch, int rows,
                                                                   bool pairs, void* out, long long row16, int* status) {
@@ -125,20 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
   grid_wait_previous();
   grid_allow_next();
   if (blockIdx.x == 0 && batch <= 32) {
-    const int lane = threadIdx.x & 31;
-    const int start = lane < batch ? ld_global(cu_seqlens + lane) : 0, end = lane < batch ? ld_global(cu_seqlens + lane + 1) : 0;
-    const bool ok = __all_sync(0xffffffffu, start >= 0 && end >= start && end <= rows);
-    int counts[2] = {0, 0};
-    if (ok) {
-      counts[0] = write_short_list(start, end - start, 1, plan.tiles);
-      if (pairs) counts[1] = write_short_list(start, end - start, 2, plan.pairs);
-    }
-    if (threadIdx.x == 0) {
-      plan.counts[0] = counts[0];
-      plan.counts[1] = counts[1];
-    plan.counts[2] = 0;
-      if (!ok) atomicCAS(status, 0, kStatusSequences);
-    }
+    write_short_plan(ShortBatch(cu_seqlens, batch, rows), plan, pairs, threadIdx.x >> 5, kPlanThreads / 32, status);
     return;
   }
   const bool ok = sequences_ok(cu_seqlens, batch, rows);

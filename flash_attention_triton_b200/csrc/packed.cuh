@@ -64,7 +64,10 @@ constexpr int kStatusSequences = 0x80000;
 
 cudaError_t launch_packed_plan(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, bool pairs, void* out,
                                int* status, int num_sms, cudaStream_t stream);
-cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+// Whether every work item of the forward has a CTA of its own.  It then reads cu_seqlens itself, writes the plan for
+// the backward and clears what launch_packed_plan would, and there is no launch in front of it: 2.5 us less on the host, 3 on the GPU.
+bool packed_fwd_alone(const PackedShape& s, int num_sms);
+cudaError_t launch_packed_fwd(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                               const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms,
                               cudaStream_t stream);
 cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& plan, const int* cu_seqlens, const void* o,
@@ -105,6 +108,63 @@ inline cudaError_t launch_dependent_cluster(void (*kernel)(Params...), unsigned 
 __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   const uint4 v = ld_global(reinterpret_cast<const uint4*>(p));
   return PackedTile{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w)};
+}
+
+// Up to 32 sequences, one a lane (whole warp).
+struct ShortBatch {
+  int start, length;  // of this lane's sequence; all lengths 0 where cu_seqlens fall or leave the rows
+  int base;           // tiles of the sequences before it
+  bool ok;
+  int first, last;    // rows that the sequences cover
+  __device__ __forceinline__ ShortBatch(const int* cu_seqlens, int batch, int rows) {
+    const int lane = threadIdx.x & 31;
+    start = lane < batch ? ld_global(cu_seqlens + lane) : 0;
+    const int end = lane < batch ? ld_global(cu_seqlens + lane + 1) : 0;
+    ok = __all_sync(0xffffffffu, start >= 0 && end >= start && end <= rows);
+    first = ok ? __shfl_sync(0xffffffffu, start, 0) : rows;
+    last = ok ? __shfl_sync(0xffffffffu, end, batch - 1) : rows;
+    length = ok ? end - start : 0;
+    base = (length + 127) >> 7;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, base, o);
+      if (lane >= o) base += y;
+    }
+    base -= (length + 127) >> 7;
+  }
+};
+
+// Entry t of a sequence comes behind those of higher numbers in all sequences and those of the same number in the sequences
+// before it, which each of the `warps` warps counts without a word to the others.
+__device__ __forceinline__ int write_short_list(const ShortBatch& s, int per, PackedTile* list, int warp, int warps) {
+  const int lane = threadIdx.x & 31;
+  const int tiles = (s.length + 127) >> 7, n = (tiles + per - 1) / per;
+  const int most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n));
+  for (int t = warp; t < most; t += warps) {
+    const int higher = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - t - 1, 0)));
+    const unsigned same = __ballot_sync(0xffffffffu, n > t);
+    if (n > t)
+      *reinterpret_cast<int4*>(list + higher + __popc(same & ((1u << lane) - 1u))) = make_int4(s.start, s.length, t * per, s.base);
+  }
+  return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
+}
+
+__device__ __forceinline__ void write_short_plan(const ShortBatch& s, const PackedPlan& plan, bool pairs, int warp, int warps, int* status) {
+  const int tiles = write_short_list(s, 1, plan.tiles, warp, warps), two = pairs ? write_short_list(s, 2, plan.pairs, warp, warps) : 0;
+  if (warp == 0 && (threadIdx.x & 31) == 0) {
+    plan.counts[0] = tiles;
+    plan.counts[1] = two;
+    plan.counts[2] = 0;
+    if (!s.ok) atomicCAS(status, 0, kStatusSequences);
+  }
+}
+
+// Zeros in the rows of a dense [rows, row16 * 8] tensor that no sequence has.
+__device__ __forceinline__ void clear_outside(void* out, long long row16, int first, int last, int rows, long long worker, long long workers) {
+  if (out == nullptr) return;
+  uint4* const p = static_cast<uint4*>(out);
+  for (long long i = worker; i < first * row16; i += workers) p[i] = make_uint4(0, 0, 0, 0);
+  for (long long i = last * row16 + worker; i < rows * row16; i += workers) p[i] = make_uint4(0, 0, 0, 0);
 }
 
 // Clears rows `first` .. ROWS - 1 of a staged [ROWS, D] tile (whole warp; nothing where first >= ROWS) before a product sums

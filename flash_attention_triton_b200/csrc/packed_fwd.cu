@@ -68,8 +68,8 @@ template <int D, bool BF16, int KD>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, uint16_t* out, float* lse,
-                      int* counts, const PackedTile* list, int rows, int Hq, int G, int cols, bool two_heads,
-                      float scale_log2, int* status) {
+                      const int* cu_seqlens, const __grid_constant__ PackedPlan plan, bool alone, int rows, int batch, int Hq, int G,
+                      int cols, bool two_heads, float scale_log2, int* status) {
   using C = PackedFwdCfg<D>;
   using T = Tile<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -142,13 +142,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&tv);
       }
       const int per_tile = two_heads ? Hq / 2 : Hq;  // items of a list entry
-      const int total_items = ld_global(counts + (two_heads ? 0 : 1)) * per_tile;
+      const PackedTile* const list = two_heads ? plan.tiles : plan.pairs;
+      const int per = two_heads ? 1 : 2;  // tiles of an entry
+      PackedTile own{0, 0, 0, 0};         // the entry of a CTA that has one item
+      int entries;
+      if (alone) {
+        const ShortBatch s(cu_seqlens, batch, rows);
+        const int mine = ((s.length + 127) / 128 + per - 1) / per;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        entries = __shfl_sync(0xffffffffu, upto, 31);
+        const int entry = blockIdx.x / per_tile;
+        if (entry < entries) {
+          const int l = __ffs(__ballot_sync(0xffffffffu, upto > entry)) - 1;
+          own = PackedTile{__shfl_sync(0xffffffffu, s.start, l), __shfl_sync(0xffffffffu, s.length, l),
+                           (entry - __shfl_sync(0xffffffffu, upto - mine, l)) * per, 0};
+        }
+      } else {
+        entries = ld_global(plan.counts + (two_heads ? 0 : 1));
+      }
+      const int total_items = entries * per_tile;
       bool ok = true;
       int ks = 0, kph = 0, vs = 0, vph = 0;  // ring positions
       int drawn = blockIdx.x;                // an item, or total_items or more: there is none
       const bool draws = total_items > static_cast<int>(gridDim.x);
       auto draw = [&]() {
-        if (lane == 0) drawn = draws ? atomicAdd(counts + 2, 1) : total_items;
+        if (lane == 0) drawn = draws ? atomicAdd(plan.counts + 2, 1) : total_items;
       };
       auto drawn_item = [&]() {  // the number drawn, for the whole warp
         if (lane == 0) *next_slot = drawn;
@@ -163,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         PackedItem item{0, 0, {-1, -1}, {0, 0}, {0, 0}};
         if (id < total_items) {
           const int entry = id / per_tile, h = id - entry * per_tile;
-          const PackedTile e = load_tile(list + entry);
+          const PackedTile e = alone ? own : load_tile(list + entry);
           const bool second = two_heads || e.tile * 128 + 128 < e.length;
           item = PackedItem{e.row0, e.length, {e.tile, second ? e.tile + (two_heads ? 0 : 1) : -1},
                             {two_heads ? 2 * h : h, two_heads ? 2 * h + 1 : h}, {0, 0}};
@@ -288,6 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+    } else if (alone) {
+      // ---------------------------------------------------------------- warp 11, where there is no plan kernel
+      const ShortBatch s(cu_seqlens, batch, rows);
+      if (blockIdx.x == 0) write_short_plan(s, plan, !two_heads, 0, 1, status);
+      clear_outside(out, static_cast<long long>(Hq) * cols / 8, s.first, s.last, rows, blockIdx.x * 32ll + lane, gridDim.x * 32ll);
     }
     __syncwarp();
   } else {
@@ -447,29 +475,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Work items at most.
+long long most_items(const PackedShape& s) {
+  return static_cast<long long>(packed_capacity(s.rows, s.batch)) * (s.Hq / s.Hkv % 2 == 0 ? s.Hq / 2 : s.Hq);
+}
+
 template <int D, bool BF16, int KD = D>
-cudaError_t launch_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+cudaError_t launch_t(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                      const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms, cudaStream_t stream) {
   using C = PackedFwdCfg<D>;
   auto kern = packed_fwd_kernel<D, BF16, KD>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   const bool two_heads = s.Hq / s.Hkv % 2 == 0;
-  const long long items = static_cast<long long>(plan.capacity) * (two_heads ? s.Hq / 2 : s.Hq);
+  const long long items = most_items(s);
   const unsigned grid = static_cast<unsigned>(items < num_sms ? items : num_sms);
-  return launch_dependent(kern, grid, kThreads, C::kSmemBytes, stream, tq, tk, tv, to, static_cast<uint16_t*>(out), lse, plan.counts,
-                          two_heads ? plan.tiles : plan.pairs, s.rows, s.Hq, s.Hq / s.Hkv, s.Dg, two_heads,
+  return launch_dependent(kern, grid, kThreads, C::kSmemBytes, stream, tq, tk, tv, to, static_cast<uint16_t*>(out), lse, cu_seqlens, plan,
+                          packed_fwd_alone(s, num_sms), s.rows, s.batch, s.Hq, s.Hq / s.Hkv, s.Dg, two_heads,
                           s.scale * 1.4426950408889634f, status);
 }
 
 }  // namespace
 
-cudaError_t launch_packed_fwd(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
+bool packed_fwd_alone(const PackedShape& s, int num_sms) { return s.batch <= 32 && most_items(s) <= num_sms; }
+
+cudaError_t launch_packed_fwd(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                               const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms,
                               cudaStream_t stream) {
 #define FA2_CASE(DD, KK)                                                                          \
-  return s.dtype ? launch_t<DD, true, KK>(s, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)  \
-                 : launch_t<DD, false, KK>(s, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)
+  return s.dtype ? launch_t<DD, true, KK>(s, cu_seqlens, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)  \
+                 : launch_t<DD, false, KK>(s, cu_seqlens, plan, tq, tk, tv, to, out, lse, status, num_sms, stream)
   if (s.D == 32) FA2_CASE(32, 32);
   if (s.D == 64) FA2_CASE(64, 64);
   if (s.Dg <= kShortDim128) FA2_CASE(128, kShortDim128);
