@@ -504,78 +504,71 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
   }
 }
 
-// Adds up the parts of what decode_kernel's stretches cut apart: block (c, row) one query head of Cut c.  First the weights of all parts, one a thread, then the parts, D / 2 threads to each, so that no load waits for
-// another.  Few long sequences have a hundred parts and more to a head: one thread a column, part after part, took
-// 73 us on two sequences of 131072 keys.
-constexpr int kJoinThreads = 256;
+// Adds up the parts of what decode_kernel's stretches cut apart: block (c, row) one query head of Cut c.  Shares of D / 2 threads
+// take every n-th part, several at a time with their maxima and sums, so that a share waits for memory once for
+// kJoinBatch parts; then the shares become one.  Few long sequences have a hundred parts and more to a head: one thread a
+// column, part after part, took 73 us on two sequences of 131 072 keys, weights first and the parts behind them 13.5.
+constexpr int kJoinMost = 512, kJoinBatch = 8;
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass_heads,
-                                                                   int hp, int slots, int ctas) {
-  __shared__ float weight[kJoinThreads], reduced[kJoinThreads / 32];
-  __shared__ float2 sums[kJoinThreads];
+__global__ void __launch_bounds__(kJoinMost) decode_join_kernel(const __grid_constant__ DecodeArgs a, int rows, int pass_heads, int hp,
+                                                                int slots, int ctas) {
+  __shared__ float4 shared[kJoinMost];  // sums of two columns, maximum, sum of the weights
   grid_wait_previous();
   grid_allow_next();
   const Workspace space(a.workspace, slots, ctas);
-  const int place_rows = hp * rows;
+  const int place_rows = hp * rows, row = blockIdx.x % place_rows;
   const uint4 c = ld_global(reinterpret_cast<const uint4*>(space.cuts) + blockIdx.x / place_rows);
   const Cut cut{static_cast<int>(c.x), static_cast<int>(c.y), static_cast<int>(c.z), static_cast<int>(c.w)};
-  const int row = blockIdx.x % place_rows;
   const int group = a.Hq / a.Hkv, blocks = (group + pass_heads - 1) / pass_heads, pass = blockIdx.x / place_rows % blocks;
   const int in_group = pass * pass_heads + row % rows;
   if (cut.last < 0 || in_group >= group) return;
   const int parts = cut.last - cut.first + 1, d2 = a.D / 2;
-  const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = kJoinThreads / d2;
-  auto cta = [&](int i) { return (cut.first + i) * blocks + pass; };
-  auto part = [&](int i) { return space.part(2 * cta(i) + (i == 0 ? 1 : 0), place_rows, a.D); };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = threadIdx.x % d2, share = threadIdx.x / d2, shares = blockDim.x / d2;
   float top = -INFINITY, all = 0.f;
   float2 sum = make_float2(0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += kJoinThreads) {
-    const int here = min(parts - p0, kJoinThreads);
-    float m = -INFINITY, l = 0.f;
-    // a CTA without units (there are fewer units than CTAs) has left nothing
-    if (threadIdx.x < here && ld_global(space.counts + cta(p0 + threadIdx.x)) != 0) {
-      const float* const at = part(p0 + threadIdx.x) + 2 * row;
-      m = ld_global(at), l = ld_global(at + 1);
-    }
-    float most = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) reduced[warp] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) most = fmaxf(most, reduced[i]);
-    most = fmaxf(most, top);
-    const float old = part_weight(top, all, most, a.scale_log2);
+  auto add = [&](float m, float l, float2 x, float now) {
+    const float f = part_weight(m, l, now, a.scale_log2);
+    all = fmaf(f, l, all);
+    // (weight 0: the part may have been left out, and hold anything)
+    sum.x = f == 0.f ? sum.x : fmaf(f, x.x, sum.x);
+    sum.y = f == 0.f ? sum.y : fmaf(f, x.y, sum.y);
+  };
+  auto lower = [&](float now) {
+    const float old = part_weight(top, all, now, a.scale_log2);
     all *= old, sum.x *= old, sum.y *= old;
-    top = most;
-    const float w = part_weight(m, l, top, a.scale_log2);
-    weight[threadIdx.x] = w;
-    l *= w;
+    top = now;
+  };
+  if (share < shares)
+    for (int i0 = share; i0 < parts; i0 += kJoinBatch * shares) {
+      float2 ml[kJoinBatch], x[kJoinBatch];
+      int some[kJoinBatch];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    __syncthreads();
-    if (lane == 0) reduced[warp] = l;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kJoinThreads / 32; ++i) all += reduced[i];
-    if (share < shares)
-#pragma unroll 8
-      for (int i = share; i < here; i += shares) {
-        const float f = weight[i];
-        const float2 x = ld_global(reinterpret_cast<const float2*>(part(p0 + i) + 2 * place_rows + row * a.D + 2 * col));
-        // (weight 0: the part may have been left out, and hold anything)
-        sum.x = f == 0.f ? sum.x : fmaf(f, x.x, sum.x);
-        sum.y = f == 0.f ? sum.y : fmaf(f, x.y, sum.y);
+      for (int j = 0; j < kJoinBatch; ++j) {
+        const int i = min(i0 + j * shares, parts - 1), cta = (cut.first + i) * blocks + pass;
+        const float* const at = space.part(2 * cta + (i == 0 ? 1 : 0), place_rows, a.D);
+        // a CTA without units (there are fewer units than CTAs) has left nothing
+        some[j] = i0 + j * shares < parts ? ld_global(space.counts + cta) : 0;
+        ml[j] = ld_global(reinterpret_cast<const float2*>(at + 2 * row));
+        x[j] = ld_global(reinterpret_cast<const float2*>(at + 2 * place_rows + row * a.D + 2 * col));
       }
-    __syncthreads();
-  }
-  sums[threadIdx.x] = sum;
+      float now = top;
+#pragma unroll
+      for (int j = 0; j < kJoinBatch; ++j) {
+        if (!some[j]) ml[j] = make_float2(-INFINITY, 0.f);
+        now = fmaxf(now, ml[j].x);
+      }
+      lower(now);
+#pragma unroll
+      for (int j = 0; j < kJoinBatch; ++j) add(ml[j].x, ml[j].y, x[j], now);
+    }
+  shared[threadIdx.x] = make_float4(sum.x, sum.y, top, all);
   __syncthreads();
   if (share == 0) {
     for (int i = 1; i < shares; ++i) {
-      const float2 x = sums[i * d2 + col];
-      sum.x += x.x, sum.y += x.y;
+      const float4 x = shared[i * d2 + col];
+      const float now = fmaxf(top, x.z);
+      lower(now);
+      add(x.z, x.w, make_float2(x.x, x.y), now);
     }
     const float inv = 1.f / all;  // NaN for a row without any finite score, as everywhere
     uint16_t* const to = static_cast<uint16_t*>(a.out) + (static_cast<long long>(cut.b) * a.Hq + (cut.h * hp + row / rows) * group + in_group) * a.D + 2 * col;
@@ -614,8 +607,10 @@ cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const 
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;
-  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows * HP, kJoinThreads, 0, stream, a, g.rows, 8 * NT, HP,
-                          g.cuts, g.ctas);
+  // as many shares as take the parts of a cut at once, were the cuts alike
+  const int batches = (g.ctas / g.cuts + kJoinBatch) / kJoinBatch;
+  const int threads = std::min(std::max(256, (a.D / 2 * batches + 31) / 32 * 32), kJoinMost);
+  return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows * HP, threads, 0, stream, a, g.rows, 8 * NT, HP, g.cuts, g.ctas);
 }
 
 }  // namespace
