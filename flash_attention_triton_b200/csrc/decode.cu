@@ -12,7 +12,7 @@
 //
 // Inside a CTA warp w takes keys 16 w .. 16 w + 15 of every unit and runs on its own: tiled copies bring its keys and
 // values into a ring of stages of its own, as many rows to a copy as 16 keys have next to each other in a page (16 where
-// the page size is a multiple of it).  The keys are the 16 rows of m16n8k16 products and the query heads of the key
+// the page size is a multiple of it); where that is one row, the lanes bring 16 bytes each.  The keys are the 16 rows of m16n8k16 products and the query heads of the key
 // head their 8 columns: S^T = K Q^T, O^T += V^T P^T, fp32 accumulators in registers, P^T turned around by
 // movmatrix.  Eight query heads fill the product; as its rows they would fill half of it.  The four warps meet
 // where a (sequence, key head) ends, while their next stages are already loading.  The products take a fraction of
@@ -187,7 +187,16 @@ struct Workspace {
   __device__ float* part(int place, int rows, int D) const { return parts + static_cast<long long>(place) * rows * (D + 2); }
 };
 
-template <int DP, int HP, int NT, bool BF16>
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on `bar` once the copies that this thread has started have come in.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// TILED: keys and values come in tiled copies of `box_rows` rows; else (one row) 16 bytes a lane.
+template <int DP, int HP, int NT, bool BF16, bool TILED>
 __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
     decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ DecodeArgs a, int rows, int slots, int box_rows, int* status) {
@@ -211,12 +220,17 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
   const int heads = a.Hkv / HP, d8 = a.D / 8;
 
   if (lane == 0)
-    for (int s = 0; s < C::kStages; ++s) mbar_init(bar(s), 1);
+    for (int s = 0; s < C::kStages; ++s) mbar_init(bar(s), TILED ? 1 : 32);
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    prefetch_tensormap(&tk);
-    prefetch_tensormap(&tv);
+    if constexpr (TILED) {
+      prefetch_tensormap(&tk);
+      prefetch_tensormap(&tv);
+    }
   }
+  if constexpr (!TILED)  // columns beyond the head dim, which no copy touches
+    for (int i = lane; i < C::kWarpBytes / 16; i += 32)
+      *reinterpret_cast<uint4*>(smem + warp * C::kWarpBytes + i * 16) = make_uint4(0, 0, 0, 0);
   fence_mbar_init();
   fence_proxy_async_smem();
   __syncthreads();
@@ -270,17 +284,36 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
     keys = __reduce_or_sync(0xffffffffu, keys);
     if (copies != 0) {
       const uint32_t dst = ring + stage * 2 * C::kTileBytes;
-      if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * C::kWide * 4);
-      __syncwarp();
-      if (take) {
+      if constexpr (TILED) {
+        if (lane == 0) mbar_arrive_expect_tx(bar(stage), copies * box_rows * C::kWide * 4);
+        __syncwarp();
+        if (take) {
 #pragma unroll
-        for (int ch = 0; ch < C::kChunks; ++ch) {
-          const uint32_t to = dst + ch * 2048 + lane * box_rows * 128;
-          const int x = HP == 2 ? 0 : ch * 64;
-          const HeadCoord from{HP == 2 ? 2 * load.h + ch : load.h, page};
-          tma_load_4d(to, &tk, x, slot, from, bar(stage));
-          tma_load_4d(to + C::kTileBytes, &tv, x, slot, from, bar(stage));
+          for (int ch = 0; ch < C::kChunks; ++ch) {
+            const uint32_t to = dst + ch * 2048 + lane * box_rows * 128;
+            const int x = HP == 2 ? 0 : ch * 64;
+            const HeadCoord from{HP == 2 ? 2 * load.h + ch : load.h, page};
+            tma_load_4d(to, &tk, x, slot, from, bar(stage));
+            tma_load_4d(to + C::kTileBytes, &tv, x, slot, from, bar(stage));
+          }
         }
+      } else {
+        // lane i has piece i % kPieces of every (32 / kPieces)-th row; columns beyond the head dim stay the zeros that they are
+        constexpr int kPieces = C::kWide / 8;
+        const int piece = lane % kPieces, chunk = piece / 8, column = HP == 2 ? piece % 8 : piece;
+        const long long kh = (HP == 2 ? 2 * load.h + chunk : load.h) * a.sk_cache.head + column * 8;
+        const long long vh = (HP == 2 ? 2 * load.h + chunk : load.h) * a.sv_cache.head + column * 8;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += 32 / kPieces) {
+          const int row = r0 + lane / kPieces, p = __shfl_sync(0xffffffffu, take ? page : -1, row);
+          const long long at = __shfl_sync(0xffffffffu, slot, row);
+          if (p >= 0 && column < d8) {
+            const uint32_t to = dst + chunk * 2048 + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+            copy16(to, static_cast<const uint16_t*>(a.k_cache) + p * a.sk_cache.page + at * a.sk_cache.slot + kh);
+            copy16(to + C::kTileBytes, static_cast<const uint16_t*>(a.v_cache) + p * a.sv_cache.page + at * a.sv_cache.slot + vh);
+          }
+        }
+        copies_arrive(bar(stage));
       }
     }
     next_unit(a, heads, load);
@@ -588,11 +621,11 @@ DecodeGrid decode_grid(int batch, int Hq, int Hkv, int D, int table_width, int p
   return DecodeGrid{hp, std::min(group, take), ctas, static_cast<int>(std::min<long long>(segments, ctas))};
 }
 
-template <int DP, int HP, int NT, bool BF16>
-cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int box_rows, int num_sms, int* status,
+template <int DP, int HP, int NT, bool BF16, bool TILED>
+cudaError_t launch_decode_s(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int box_rows, int num_sms, int* status,
                             cudaStream_t stream) {
   using C = DecodeCfg<DP, HP>;
-  auto kern = decode_kernel<DP, HP, NT, BF16>;
+  auto kern = decode_kernel<DP, HP, NT, BF16, TILED>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   const DecodeGrid g = decode_grid(a.batch, a.Hq, a.Hkv, a.D, a.table_width, a.page_size, std::min(num_sms * C::kCtasPerSm, kMaxCtas));
@@ -611,6 +644,16 @@ cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const 
   const int batches = (g.ctas / g.cuts + kJoinBatch) / kJoinBatch;
   const int threads = std::min(std::max(256, (a.D / 2 * batches + 31) / 32 * 32), kJoinMost);
   return launch_dependent(decode_join_kernel<BF16>, static_cast<unsigned>(g.cuts) * g.rows * HP, threads, 0, stream, a, g.rows, 8 * NT, HP, g.cuts, g.ctas);
+}
+
+// With one row to a box the tiled copies themselves bound the kernel.  64 sequences of 204 000 keys, 32 / 8 heads of 128 columns,
+// microseconds with tiled copies / 16 bytes a lane, pages of 1: 309 / 219, 2: 216 / 217, 4: 164 / 212, 8: 148 / 211; of
+// 131 000 keys, 16 / 2 heads of 256 columns, pages of 1: 171 / 106, 2: 116 / 107, 4: 84 / 105.
+template <int DP, int HP, int NT, bool BF16>
+cudaError_t launch_decode_t(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a, int box_rows, int num_sms, int* status,
+                            cudaStream_t stream) {
+  return box_rows > 1 ? launch_decode_s<DP, HP, NT, BF16, true>(tk, tv, a, box_rows, num_sms, status, stream)
+                      : launch_decode_s<DP, HP, NT, BF16, false>(tk, tv, a, box_rows, num_sms, status, stream);
 }
 
 }  // namespace

@@ -177,6 +177,14 @@ def test_decode_pages(page, layout):
     check_decode([1, 2, 3, 64, 99, 100, 101, 257], page, 4, 2, 64, BF16, layout)
 
 
+@pytest.mark.parametrize("page", [1, 2, 7])
+@pytest.mark.parametrize("heads,kv_heads,d,dtype", [(4, 2, 64, BF16), (3, 1, 40, FP16), (4, 2, 24, BF16), (4, 2, 128, FP16), (16, 1, 72, BF16),
+                                                    (2, 2, 256, BF16), (9, 1, 200, FP16)])
+def test_decode_pages_of_odd_and_small_size(page, heads, kv_heads, d, dtype):
+    """Pages of odd size come in another way, whatever else is the same."""
+    check_decode([1, 0, 63, 64, 65, 300], page, heads, kv_heads, d, dtype)
+
+
 @pytest.mark.parametrize("held", [[1], [900], [40000], [1, 20000, 0, 3], [0, 0, 0], [5000] * 7, list(range(200)), [17] * 600])
 def test_decode_lengths(held):
     check_decode(held, 16, 8, 2, 64, BF16)
