@@ -98,6 +98,43 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(const int* cu
     write_short_plan(ShortBatch(cu_seqlens, batch, rows), plan, pairs, threadIdx.x >> 5, kPlanThreads / 32, status);
     return;
   }
+  constexpr int kSome = 8;  // sequences of a lane
+  if (blockIdx.x == 0 && batch <= 32 * kSome) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int start[kSome], length[kSome], base[kSome], before = 0;
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) {
+      const int b = k * 32 + lane;
+      start[k] = b < batch ? ld_global(cu_seqlens + b) : 0;
+      length[k] = b < batch ? ld_global(cu_seqlens + b + 1) : 0;  // its end, as yet
+    }
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) ok &= start[k] >= 0 && length[k] >= start[k] && length[k] <= rows;
+    ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+    for (int k = 0; k < kSome; ++k) {
+      length[k] = ok ? length[k] - start[k] : 0;
+      const int tiles = (length[k] + 127) >> 7;
+      int upto = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      base[k] = before + upto - tiles;
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const int tiles = write_list_by_ballots<kSome>(start, length, base, 1, plan.tiles, warp, kPlanThreads / 32);
+    const int two = pairs ? write_list_by_ballots<kSome>(start, length, base, 2, plan.pairs, warp, kPlanThreads / 32) : 0;
+    if (threadIdx.x == 0) {
+      plan.counts[0] = tiles;
+      plan.counts[1] = two;
+      plan.counts[2] = 0;
+      if (!ok) atomicCAS(status, 0, kStatusSequences);
+    }
+    return;
+  }
   const bool ok = sequences_ok(cu_seqlens, batch, rows);
   if (blockIdx.x > 0) {
     const int first = ok ? ld_global(cu_seqlens) : rows, last = ok ? ld_global(cu_seqlens + batch) : rows;

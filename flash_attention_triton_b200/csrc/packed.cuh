@@ -110,6 +110,35 @@ __device__ __forceinline__ PackedTile load_tile(const PackedTile* p) {
   return PackedTile{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w)};
 }
 
+// A list of entries of `per` tiles each, those that start at the highest tiles first, for up to 32 SEQUENCES sequences, as many
+// to a lane: entry t of a sequence comes behind those of higher numbers in all sequences and those of the same number in the
+// sequences before it, which each of the `warps` warps counts without a word to the others.  Returns the entries.
+template <int SEQUENCES>
+__device__ __forceinline__ int write_list_by_ballots(const int (&start)[SEQUENCES], const int (&length)[SEQUENCES],
+                                                     const int (&base)[SEQUENCES], int per, PackedTile* list, int warp, int warps) {
+  const int lane = threadIdx.x & 31;
+  int n[SEQUENCES], all = 0, mine = 0;
+#pragma unroll
+  for (int k = 0; k < SEQUENCES; ++k) {
+    n[k] = ((length[k] + 127) / 128 + per - 1) / per;
+    mine = max(mine, n[k]), all += n[k];
+  }
+  const int most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(mine));
+  for (int t = warp; t < most; t += warps) {
+    int higher = 0;
+#pragma unroll
+    for (int k = 0; k < SEQUENCES; ++k) higher += max(n[k] - t - 1, 0);
+    int at = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(higher));
+#pragma unroll
+    for (int k = 0; k < SEQUENCES; ++k) {
+      const unsigned same = __ballot_sync(0xffffffffu, n[k] > t);
+      if (n[k] > t) *reinterpret_cast<int4*>(list + at + __popc(same & ((1u << lane) - 1u))) = make_int4(start[k], length[k], t * per, base[k]);
+      at += __popc(same);
+    }
+  }
+  return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(all));
+}
+
 // Up to 32 sequences, one a lane (whole warp).
 struct ShortBatch {
   int start, length;  // of this lane's sequence; all lengths 0 where cu_seqlens fall or leave the rows
@@ -134,23 +163,10 @@ struct ShortBatch {
   }
 };
 
-// Entry t of a sequence comes behind those of higher numbers in all sequences and those of the same number in the sequences
-// before it, which each of the `warps` warps counts without a word to the others.
-__device__ __forceinline__ int write_short_list(const ShortBatch& s, int per, PackedTile* list, int warp, int warps) {
-  const int lane = threadIdx.x & 31;
-  const int tiles = (s.length + 127) >> 7, n = (tiles + per - 1) / per;
-  const int most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n));
-  for (int t = warp; t < most; t += warps) {
-    const int higher = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(n - t - 1, 0)));
-    const unsigned same = __ballot_sync(0xffffffffu, n > t);
-    if (n > t)
-      *reinterpret_cast<int4*>(list + higher + __popc(same & ((1u << lane) - 1u))) = make_int4(s.start, s.length, t * per, s.base);
-  }
-  return __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
-}
-
 __device__ __forceinline__ void write_short_plan(const ShortBatch& s, const PackedPlan& plan, bool pairs, int warp, int warps, int* status) {
-  const int tiles = write_short_list(s, 1, plan.tiles, warp, warps), two = pairs ? write_short_list(s, 2, plan.pairs, warp, warps) : 0;
+  const int start[1] = {s.start}, length[1] = {s.length}, base[1] = {s.base};
+  const int tiles = write_list_by_ballots<1>(start, length, base, 1, plan.tiles, warp, warps);
+  const int two = pairs ? write_list_by_ballots<1>(start, length, base, 2, plan.pairs, warp, warps) : 0;
   if (warp == 0 && (threadIdx.x & 31) == 0) {
     plan.counts[0] = tiles;
     plan.counts[1] = two;

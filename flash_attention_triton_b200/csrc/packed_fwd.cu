@@ -3,8 +3,8 @@
 // The arithmetic, the warp roles and the tensor-memory plan are those of fwd_kernel (fwd.cu) with 128-row KV tiles:
 // a CTA has two score tiles in turn on one buffer, a softmax group for each, and two MMA-issuing warps.  What differs is the work
 // item.  Its two Q tiles are the same rows of two query heads that share a key head, so they read each K and V tile
-// once, end at the same KV tile, and a sequence of one tile still fills both; with an odd number of query heads to a
-// key head they are two adjacent tiles of one head.  The items come from the plan, heaviest first, all heads of a tile
+// once, end at the same KV tile, and a sequence of one tile still fills both.  With an odd number G of query heads to a
+// key head the 2 G (tile, head) of two adjacent tiles make G items; one of them has either tile.  The items come from the plan, heaviest first, all heads of a tile
 // one after the other (their K and V pass the L2 together).  Bound by the tensor pipe at head dim 128, by the
 // exponentials below, like fwd_kernel.
 #include "mma_issue.cuh"
@@ -187,9 +187,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (id < total_items) {
           const int entry = id / per_tile, h = id - entry * per_tile;
           const PackedTile e = alone ? own : load_tile(list + entry);
-          const bool second = two_heads || e.tile * 128 + 128 < e.length;
-          item = PackedItem{e.row0, e.length, {e.tile, second ? e.tile + (two_heads ? 0 : 1) : -1},
-                            {two_heads ? 2 * h : h, two_heads ? 2 * h + 1 : h}, {0, 0}};
+          if (two_heads) {
+            item = PackedItem{e.row0, e.length, {e.tile, e.tile}, {2 * h, 2 * h + 1}, {0, 0}};
+          } else {
+            // the two of number x and x + 1 among the (tile, head) of the entry and key head, tile by tile
+            const int kv_head = h / G, x = 2 * (h - kv_head * G), there = e.tile * 128 + 128 < e.length ? 2 * G : G;
+            if (x >= there) {  // the entry has one tile, and the items before this one have taken it
+              draw();
+              --n;
+              continue;
+            }
+            const int t0 = x >= G, t1 = x + 1 >= G, head = kv_head * G + x;
+            item = PackedItem{e.row0, e.length, {e.tile + t0, x + 1 < there ? e.tile + t1 : -1}, {head - t0 * G, head + 1 - t1 * G}, {0, 0}};
+          }
         }
         if (ok) ok = mbar_wait_warp(bar(C::kBarItemEmpty + (n & 1)), ((n >> 1) & 1) ^ 1, w, kSiteItem);
         if (ok && lane == 0) {
