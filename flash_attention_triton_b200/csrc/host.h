@@ -25,13 +25,21 @@ void check_status_if_asked(const char* fn, const at::Tensor& on);
 inline int dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FA2_DTYPE_FP16 : FA2_DTYPE_BF16; }
 inline bool is_16bit(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 
-// A tensor argument, or an undefined one for None where that is allowed; TypeError for anything else.
+// A tensor argument, or an undefined one for None where that is allowed; TypeError for anything else.  What stands for
+// another tensor (in a transform, under a fake-tensor mode) or carries a forward-mode tangent is refused, not computed without it.
 inline at::Tensor tensor_argument(PyObject* arg, const char* name, bool optional = false) {
   if (optional && arg == Py_None) return {};
   TORCH_CHECK_TYPE(THPVariable_Check(arg), name, " must be a tensor", optional ? " or None" : "");
   const at::Tensor& t = THPVariable_Unpack(arg);
   TORCH_CHECK_VALUE(t.defined() && t.layout() == at::kStrided, name, " must be a dense tensor");
+  TORCH_CHECK_VALUE(t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch() && !t._fw_grad(0).defined(), name,
+                    " must be a plain tensor: there is no form for transforms, fake tensors and forward-mode differentiation");
   return t.is_neg() ? t.resolve_neg() : t;
+}
+// A tensor that the call writes: not a view that negates what it shows.
+inline at::Tensor written_argument(PyObject* arg, const char* name) {
+  TORCH_CHECK_VALUE(!THPVariable_Check(arg) || !THPVariable_Unpack(arg).is_neg(), name, " must not be a negating view");
+  return tensor_argument(arg, name);
 }
 
 // The softmax scale of a call: None and 0.0 mean 1 / sqrt(head dim).

@@ -75,7 +75,7 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (nargs != 12) return PyErr_Format(PyExc_TypeError, "kv_append takes 12 arguments");
   at::Tensor k = tensor_argument(args[0], "k"), v = tensor_argument(args[1], "v");
-  const at::Tensor k_cache = tensor_argument(args[2], "k_cache"), v_cache = tensor_argument(args[3], "v_cache");
+  const at::Tensor k_cache = written_argument(args[2], "k_cache"), v_cache = written_argument(args[3], "v_cache");
   const at::Tensor table = tensor_argument(args[4], "block_table"), lengths = tensor_argument(args[5], "lengths");
   const at::Tensor cu_seqlens = tensor_argument(args[6], "cu_seqlens", true);
   at::Tensor q = tensor_argument(args[7], "q", true);

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_allow_next();
 
   // Slot of the n-th item of this CTA, for every role but the producer; false: there is none, or the CTA gives up.
-  // It votes; the MMA warps' other waits do not, see fwd_kernel.
+  // It votes; the other waits of the warp that issues S do not, see fwd_kernel.
   auto take_item = [&](int n, PackedItem& item) {
     if (!mbar_wait_warp(bar(C::kBarItemFull + (n & 1)), (n >> 1) & 1, w, kSiteItem)) return false;
     item = reinterpret_cast<const PackedItem*>(smem + C::kOffItems)[n & 1];
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int n = 0; ok && take_item(n, item); ++n) {
         const int n0 = kv_tiles(item, 0), n1 = kv_tiles(item, 1), nkv = max(n0, n1);
         for (int j = 0; ok && j < nkv; ++j) {
-          // the only wait of this warp that votes besides take_item: clear_rows wants it converged
+          // the waits of this warp vote: clear_rows wants it converged
           if (!(ok = mbar_wait_warp(bar(C::kBarVFull + vs), vph, w, kSiteMmaV))) break;
           clear_rows<D, 128>(smem + C::kOffV + vs * T::kTileBytes, item.length - j * 128, lane);
 #pragma unroll

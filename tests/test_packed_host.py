@@ -90,3 +90,16 @@ def test_formulas_of_the_gradients_against_differences():
                 ends.append((o * do).sum().item())
             # central differences: step^2 times a third derivative, 1e-16 / step of the sums' roundings
             assert abs((ends[0] - ends[1]) / (2 * step) - exact[name][index].item()) < 1e-8
+
+
+def test_transforms_and_tangents_are_refused():
+    """A tangent would be lost in silence otherwise."""
+    import torch.autograd.forward_ad as fwad
+
+    a = arguments()
+    with fwad.dual_level(), pytest.raises(ValueError, match="q must be a plain tensor"):
+        fa.flash_attention_packed(**{**a, "q": fwad.make_dual(a["q"], torch.ones_like(a["q"]))})
+    with pytest.raises(ValueError, match="v must be a plain tensor"):
+        torch.func.grad(lambda v: fa.flash_attention_packed(**{**a, "v": v}).float().sum())(a["v"])
+    with pytest.raises(ValueError, match="q must be a plain tensor"):
+        torch.vmap(lambda q: fa.flash_attention_packed(**{**a, "q": q}))(a["q"][None])

@@ -132,3 +132,13 @@ def test_rotary_tables():
     assert abs(cos[p, j].item() - math.cos(angle)) < 1e-7 and abs(sin[p, j].item() - math.sin(angle)) < 1e-7
     with pytest.raises(ValueError, match="multiple of 16"):
         fa.rotary_tables(10, 24)
+
+
+def test_a_cache_that_cannot_be_written_is_refused():
+    """The copy that stands for a negating view would be written in its place."""
+    a = append_arguments()
+    for name in ("k_cache", "v_cache"):
+        with pytest.raises(ValueError, match=f"{name} must not be a negating view"):
+            fa.append_kv_cache(**{**a, name: torch._neg_view(a[name])})
+    with torch.no_grad(), pytest.raises(ValueError, match="q must be a plain tensor"):
+        torch.vmap(lambda q: fa.flash_attention_decode(**{**decode_arguments(), "q": q}))(decode_arguments()["q"][None])
