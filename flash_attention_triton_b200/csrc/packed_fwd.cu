@@ -147,34 +147,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int per_tile = two_heads ? Hq / 2 : Hq;  // items of a list entry
       const PackedTile* const list = two_heads ? plan.tiles : plan.pairs;
       const int per = two_heads ? 1 : 2;  // tiles of an entry
-      PackedTile own{0, 0, 0, 0};         // the entry of a CTA that has one item
-      int entries;
+      // alone: this lane's sequence, and the entries it has in the list that there is no plan of
+      int start = 0, length = 0, mine = 0, entries;
       if (alone) {
         const ShortBatch s(cu_seqlens, batch, rows);
-        const int mine = ((s.length + 127) / 128 + per - 1) / per;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += y;
-        }
-        entries = __shfl_sync(0xffffffffu, upto, 31);
-        const int entry = blockIdx.x / per_tile;
-        if (entry < entries) {
-          const int l = __ffs(__ballot_sync(0xffffffffu, upto > entry)) - 1;
-          own = PackedTile{__shfl_sync(0xffffffffu, s.start, l), __shfl_sync(0xffffffffu, s.length, l),
-                           (entry - __shfl_sync(0xffffffffu, upto - mine, l)) * per, 0};
-        }
+        start = s.start, length = s.length, mine = ((s.length + 127) / 128 + per - 1) / per;
+        entries = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(mine));
       } else {
         entries = ld_global(plan.counts + (two_heads ? 0 : 1));
       }
       const int total_items = entries * per_tile;
+      // Entry `at` of that list, which has the order of write_list_by_ballots (whole warp).
+      auto find = [&](int at) {
+        auto from = [&](int number) { return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(max(mine - number, 0)))); };
+        int low = 0, high = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(mine)));
+        while (low + 1 < high) {
+          const int mid = (low + high) >> 1;
+          if (from(mid) > at) low = mid; else high = mid;
+        }
+        const int rank = at - from(low + 1);  // among the sequences that have an entry of number `low`
+        const unsigned same = __ballot_sync(0xffffffffu, mine > low);
+        const int l = __ffs(__ballot_sync(0xffffffffu, mine > low && __popc(same & ((1u << lane) - 1u)) == rank)) - 1;
+        return PackedTile{__shfl_sync(0xffffffffu, start, l), __shfl_sync(0xffffffffu, length, l), low * per, 0};
+      };
       bool ok = true;
       int ks = 0, kph = 0, vs = 0, vph = 0;  // ring positions
       int drawn = blockIdx.x;                // an item, or total_items or more: there is none
-      const bool draws = total_items > static_cast<int>(gridDim.x);
+      const bool draws = !alone && total_items > static_cast<int>(gridDim.x);
+      int round = 0;
       auto draw = [&]() {
-        if (lane == 0) drawn = draws ? atomicAdd(plan.counts + 2, 1) : total_items;
+        if (alone)  // to and fro through the list, so that who has the heaviest of one round has the lightest of the next
+          ++round, drawn = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        else if (lane == 0)
+          drawn = draws ? atomicAdd(plan.counts + 2, 1) : total_items;
       };
       auto drawn_item = [&]() {  // the number drawn, for the whole warp
         if (lane == 0) *next_slot = drawn;
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         PackedItem item{0, 0, {-1, -1}, {0, 0}, {0, 0}};
         if (id < total_items) {
           const int entry = id / per_tile, h = id - entry * per_tile;
-          const PackedTile e = alone ? own : load_tile(list + entry);
+          const PackedTile e = alone ? find(entry) : load_tile(list + entry);
           if (two_heads) {
             item = PackedItem{e.row0, e.length, {e.tile, e.tile}, {2 * h, 2 * h + 1}, {0, 0}};
           } else {
@@ -510,7 +515,12 @@ cudaError_t launch_t(const PackedShape& s, const int* cu_seqlens, const PackedPl
 
 }  // namespace
 
-bool packed_fwd_alone(const PackedShape& s, int num_sms) { return s.batch <= 32 && most_items(s) <= num_sms; }
+// Up to 32 sequences (a warp looks through them) and a few items to a CTA: who finds items alone cannot draw them, and takes a fixed share.
+// Microseconds with the plan / alone: 16 x 200 rows, 8 / 8 heads of 64 (2.2 items a CTA) 11.5 / 9.7, 4 x 512, 16 / 4 (1.1) 14.1 / 12.7,
+// eight of 256 to 1024, 16 / 4 (2.5) 25.1 / 24.9, 8 x 1024, 8 / 8 (3.9) 25.6 / 23.6, 32 x 300, 16 / 4 (5.8) 33.4 / 35.7,
+// six of 616 to 4096, 32 / 8 of 128 (8) 160 / 163.
+constexpr int kAloneRounds = 4;
+bool packed_fwd_alone(const PackedShape& s, int num_sms) { return s.batch <= 32 && most_items(s) <= kAloneRounds * num_sms; }
 
 cudaError_t launch_packed_fwd(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                               const CUtensorMap& tv, const CUtensorMap& to, void* out, float* lse, int* status, int num_sms,

@@ -350,3 +350,13 @@ def test_saved_tensor_hooks():
         k.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(o, leaves, do)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 4, 64), (9, 3, 40), (5, 5, 128), (2, 1, 32)])
+@pytest.mark.parametrize("lengths", [[700, 1, 300, 129, 640, 0, 128, 90, 1500, 2], [257] * 32, [2900, 64], [1] * 31 + [2500]])
+def test_items_found_with_and_without_a_plan(heads, kv_heads, d, lengths):
+    """With up to 32 sequences and few items the CTAs find these themselves, one or several each; with 40 a plan has them: the same bits."""
+    check(lengths, heads, kv_heads, d, BF16)
+    q, k, v, do = inputs(lengths, heads, kv_heads, d, BF16, behind=7)
+    o = run(q, k, v, cu_of(lengths))["o"]
+    assert torch.equal(o, run(q, k, v, cu_of(lengths + [0] * (40 - len(lengths))))["o"])
