@@ -10,9 +10,10 @@
 // that the rotation joins in two heads, or the same piece in four.  Their loads are in flight together, and the cosines and
 // sines are read once for all of them.  Many small CTAs: one loads while others look up places or store.  The first
 // warp of a CTA finds sequence, position and page of the CTA's tokens and leaves them in shared memory.
-// 31 323 tokens of 32 + 8 + 8 heads of 128 columns: 140 us, 91 % of the measured copy rate; with one head a thread, each token
+// 31 323 tokens of 32 + 8 + 8 heads of 128 columns: 139 us, 92 % of the measured copy rate; with one head a thread, each token
 // behind the stores of the one before, 183 us, with 512 threads to a CTA 178 us, five and six CTAs of 256 threads on an SM
-// (48 and 40 registers, spilled) 148 and 161 us.
+// (48 and 40 registers, spilled) 148 and 161 us; with the first token's loads in front of the look-up, which then waits behind
+// those of the whole SM, 184 us.
 #include <algorithm>
 
 #include "common.cuh"
@@ -100,9 +101,32 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
   grid_allow_next();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, row = first + lane;
-    int sequence = row, fresh = 1, index = 0;
+    int sequence = row, fresh = 1, index = 0, length = 0;
     bool inside = lane < count;
-    if (a.cu_seqlens != nullptr) {
+    if (a.cu_seqlens == nullptr) {
+      if (inside) length = ld_global(a.lengths + sequence);
+    } else if (a.batch <= 32) {
+      // a sequence a lane, all that there is to know about it asked for at once; each lane then finds its row's (31 323 tokens in 16
+      // prompts 141.5 -> 138.9 us, 10 855 in 12 27.3 -> 26.2 against the search below)
+      const bool there = lane < a.batch;
+      const int start = there ? ld_global(a.cu_seqlens + lane) : 0, end = there ? ld_global(a.cu_seqlens + lane + 1) : 0;
+      const int size = there ? ld_global(a.lengths + lane) : 0;
+      // the first whose end is behind the CTA's first row, and on from there
+      const unsigned behind = __ballot_sync(0xffffffffu, there && end > first);
+      sequence = behind ? __ffs(behind) - 1 : a.batch;
+      for (int s = sequence; s < a.batch; ++s) {
+        const int end_of = __shfl_sync(0xffffffffu, end, s);
+        if (inside && sequence == s && end_of <= row) ++sequence;
+        if (!__any_sync(0xffffffffu, inside && sequence > s)) break;
+      }
+      inside = inside && sequence < a.batch;
+      const int from = min(sequence, a.batch - 1);
+      const int start_of = __shfl_sync(0xffffffffu, start, from);
+      fresh = __shfl_sync(0xffffffffu, end, from) - start_of;
+      length = __shfl_sync(0xffffffffu, size, from);
+      index = row - start_of;
+      inside = inside && index >= 0;
+    } else {
       sequence = sequence_of(a.cu_seqlens, a.batch, first, lane);
       if (inside && sequence < a.batch && ld_global(a.cu_seqlens + sequence + 1) <= row) {  // a later sequence begins in between
         int low = sequence + 1, high = a.batch;
@@ -115,6 +139,7 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
       inside = inside && sequence < a.batch;
       if (inside) {
         const int start = ld_global(a.cu_seqlens + sequence);
+        length = ld_global(a.lengths + sequence);
         fresh = ld_global(a.cu_seqlens + sequence + 1) - start;
         index = row - start;
         inside = index >= 0;
@@ -122,17 +147,18 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
     }
     TokenPlace place{-1, -1, -1};
     if (inside) {
-      const long long position = static_cast<long long>(ld_global(a.lengths + sequence)) - fresh + index;
+      const long long position = static_cast<long long>(length) - fresh + index;
       if (position >= 0) {
-        const long long page_index = position / a.page_size;
+        const bool fits = position <= 0x7fffffff;  // (not where cu_seqlens fall)
+        const int p = fits ? static_cast<int>(position) : 0, page_index = p / a.page_size;
         int page = -1;
-        if (page_index < a.table_width && (a.rotary == 0 || position < a.positions))
+        if (fits && page_index < a.table_width && (a.rotary == 0 || p < a.positions))
           page = ld_global(a.block_table + sequence * a.table_stride + page_index);
         if (page >= 0 && page < a.pages) {
-          const long long slot = position - page_index * a.page_size;
+          const long long slot = p - page_index * a.page_size;
           place.k = page * a.sk_cache.page + slot * a.sk_cache.slot;
           place.v = page * a.sv_cache.page + slot * a.sv_cache.slot;
-          place.position = static_cast<int>(position);
+          place.position = p;
         } else {
           atomicCAS(status, 0, kStatusPage | kSiteAppend);
         }

@@ -79,6 +79,15 @@ def test_append_many(batch, heads, kv_heads, d):
     check_append(held, [1] * batch, 16, heads, kv_heads, d, FP16, d // 16 * 16, tokens_only=True)
 
 
+@pytest.mark.parametrize("batch", [1, 2, 31, 32, 33, 150])
+def test_append_finds_the_sequences(batch):
+    """Sequences without tokens before, between and behind those that have some; up to 32 are looked up at once."""
+    g = torch.Generator().manual_seed(batch)
+    new = [n * (torch.rand(1, generator=g).item() < 0.6) for n in torch.randint(1, 50, (batch,), generator=g).tolist()]
+    new[batch // 2] = 61
+    check_append(torch.randint(0, 40, (batch,), generator=g).tolist(), new, 16, 4, 2, 64, BF16, 64, behind=5)
+
+
 def test_append_long_prompt_and_far_positions():
     check_append([100000, 0], [300, 1500], 64, 2, 1, 64, BF16, 64)
 
