@@ -75,7 +75,7 @@ cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& pla
                                      void* dq, void* dk, void* dv, cudaStream_t stream);
 // Rows of a step of a backward kernel with `heads` CTAs to a tile, and the box height of the tensors it walks.
 int packed_step_rows(const PackedShape& s, int heads, int num_sms);
-// CTAs of the dK / dV kernel that share the query heads of a KV tile: 1, or 2 where G is even.
+// CTAs of the dK / dV kernel that share the query heads of a KV tile: 1, 2 or 4, a divisor of G.
 int packed_cluster(const PackedShape& s, int num_sms);
 cudaError_t launch_packed_dkdv(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                                const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,

@@ -78,11 +78,11 @@ __device__ __forceinline__ float group_dscale(const PackedStats& stats, int capa
 }
 
 // =========================================================================================
-// dK / dV: one CTA per KV tile of a key head, or a cluster of two (S) that share its query heads
+// dK / dV: one CTA per KV tile of a key head, or a cluster of two or four (S) that share its query heads
 // =========================================================================================
 // A KV tile with G query heads is G times the work of one, and there are G times fewer of them, so with few tiles a launch
-// waits for the longest of them.  The CTAs of a cluster then take half of the query heads each.  At their end each sends
-// its fp32 accumulators of the half of the 128 rows that the other one owns into that one's idle rings: no memory, no
+// waits for the longest of them.  The CTAs of a cluster then share the query heads, and the 128 rows.  At their end each sends
+// its fp32 accumulators of the rows that another one owns into that one's idle rings: no memory, no
 // other launch, one order of the sum.  When: packed_cluster.
 template <int D, bool BF16, int KD, int W, int S>
 __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::kCtasPerSm)
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
   grid_wait_previous();
   grid_allow_next();
 
-  static_assert(S == 1 || S == 2, "packed_cluster");
+  static_assert(S == 1 || S == 2 || S == 4, "packed_cluster");
   const int rank = S == 1 ? 0 : blockIdx.x % S, entry = blockIdx.x / S / Hkv, kv_head = blockIdx.x / S - entry * Hkv;
   const int first_head = kv_head * G + rank * (G / S);  // of this CTA's query heads
   if (entry < ld_global(counts)) {
@@ -679,6 +679,7 @@ template <int D, bool BF16, int KD, int W>
 cudaError_t launch_dkdv_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                           const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                           void* dk, void* dv, const PackedStats& stats, int cluster, int* status, cudaStream_t stream) {
+  if (cluster == 4) return launch_dkdv_s<D, BF16, KD, W, 4>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
   if (cluster == 2) return launch_dkdv_s<D, BF16, KD, W, 2>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
   return launch_dkdv_s<D, BF16, KD, W, 1>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
 }
@@ -704,13 +705,16 @@ int packed_step_rows(const PackedShape& s, int heads, int num_sms) {
   return s.D <= 64 && 100ll * packed_capacity(s.rows, s.batch) * heads >= 200ll * num_sms ? 64 : 128;
 }
 
-// Two where single CTAs would not fill the SMs one and a half times.  Whole backward, microseconds, clusters of 1 / 2 / 4:
-//   41 CTAs (16 x 200 rows, 8 / 1 heads of 128) 65.8 / 58.6 / 59.0, 130 (8192, 8 / 2 of 128) 669 / 386 / 468,
-//   192 (eight of 256 to 1024, 16 / 4 of 64) 83.3 / 74.6 / 79.0, 260 (8192, 16 / 4 of 128) 840 / 841 / 929,
-//   264 (2 x 4096, 16 / 4 of 64) 301 / 291 / 310, 272 (2 x 2048, 32 / 8 of 128) 276 / 290 / 343, 576 (8 x 1024, 32 / 8 of 128) 323 / 410 / 499.
+// Four where there are very few CTAs, two where there are few, or about as many as SMs for long sequences, whose heaviest tiles the dQ kernel cannot fill up behind.
+// Forward and backward replayed, bf16, microseconds, single CTAs / clusters, by CTAs for each SM:
+//   head dim 128, 8 / 2 heads: 8 x 512 rows (0.54) 61.2 / 61.1, 16 x 256 (0.65) 49.3 / 53.3, 4 x 1024 (0.49) 88.4 / 74.6, 8 x 1024 (0.97) 112.6 / 120.6,
+//   2 x 2048 (0.46) 146 / 105, 4 x 2048 (0.92) 158 / 166, 2 x 4096 (0.89) 268 / 264, 16 x 512 (1.08) 89 / 97.5; 2 x 8192, 8 / 1 (0.88) 1128 / 1041,
+//   2 x 2048, 32 / 1 (0.23) 837 / 462, clusters of four 293, 4096, 8 / 1 (0.22) 257 of two / 170 of four, 2 x 1024, 8 / 2 (0.24) 61.6 / 55.2,
+//   16 x 200, 32 / 1 (0.28) 128 / 129;   head dim 64: 4096, 16 / 4 (0.89) 234 / 205, eight of 256 to 1024, 16 / 4 (0.92) 62.2 / 66.7.
 int packed_cluster(const PackedShape& s, int num_sms) {
   const long long ctas = static_cast<long long>(packed_capacity(s.rows, s.batch)) * s.Hkv;
-  return s.Hq / s.Hkv % 2 == 0 && 2 * ctas <= 3ll * num_sms ? 2 : 1;
+  if (s.Hq / s.Hkv % 4 == 0 && 4 * ctas <= num_sms) return 4;
+  return s.Hq / s.Hkv % 2 == 0 && (2 * ctas <= num_sms || (ctas <= num_sms && s.rows >= 4096ll * s.batch)) ? 2 : 1;
 }
 
 #define FA2_DTYPES(CALL, DD, KK, WW) return s.dtype ? CALL<DD, true, KK, WW>(FA2_ARGS) : CALL<DD, false, KK, WW>(FA2_ARGS)

@@ -360,3 +360,11 @@ def test_items_found_with_and_without_a_plan(heads, kv_heads, d, lengths):
     q, k, v, do = inputs(lengths, heads, kv_heads, d, BF16, behind=7)
     o = run(q, k, v, cu_of(lengths))["o"]
     assert torch.equal(o, run(q, k, v, cu_of(lengths + [0] * (40 - len(lengths))))["o"])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (6, 2), (8, 2), (12, 2), (16, 1)])
+def test_query_heads_shared_by_a_cluster(dtype, d, heads, kv_heads):
+    """Four, two or one CTA to a key head's tile, by the query heads that there are."""
+    check([300, 1, 129, 0, 128, 450], heads, kv_heads, d, dtype, behind=3)

@@ -72,8 +72,8 @@ def test_forward(simulator, d, heads, kv_heads, lengths):
 @pytest.mark.parametrize("lengths", LENGTHS)
 @pytest.mark.parametrize("d,step", [(32, 64), (32, 128), (64, 64), (64, 128), (96, 128), (128, 128)])
 def test_backward(simulator, d, step, lengths):
-    for cluster in (1, 2):
-        run(simulator, "dkdv", d, 4, 2, lengths, step, cluster)
+    for cluster in (1, 2, 4):
+        run(simulator, "dkdv", d, 2 * max(2, cluster), 2, lengths, step, cluster)
     run(simulator, "dkdv", d, 3, 1, lengths, step)
     run(simulator, "dq", d, 3, 1, lengths, step)
 
