@@ -8,8 +8,8 @@
 // one after the other (their K and V pass the L2 together).  Bound by the chain of a softmax step at head dim 128, by the
 // exponentials below, like fwd_kernel.  P enters the second product in 16 bits, the type that the tensor pipe takes beside V; sums and
 // the output before its one rounding are fp32.
-// bf16, 8 808 rows in six sequences, 32 / 8 heads of 128 columns: 166 us alone (1 080 TFLOP/s, tensor pipe 63 % active), 187 a call in a
-// loop with the plan.
+// bf16, 8 808 rows in six sequences, 32 / 8 heads of 128 columns: 158 us a call in a burst (1 130 TFLOP/s, tensor pipe 63 % active), 187 in
+// a long loop, at the power limit.
 #include "mma_issue.cuh"
 #include "packed.cuh"
 
