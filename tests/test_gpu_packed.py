@@ -368,3 +368,40 @@ def test_items_found_with_and_without_a_plan(heads, kv_heads, d, lengths):
 def test_query_heads_shared_by_a_cluster(dtype, d, heads, kv_heads):
     """Four, two or one CTA to a key head's tile, by the query heads that there are."""
     check([300, 1, 129, 0, 128, 450], heads, kv_heads, d, dtype, behind=3)
+
+
+def test_calls_one_behind_the_other():
+    """Kernels of one call start under those of the call before it, in memory that calls before that one have given back."""
+    sets = [([500 + 40 * i, 3, 129], *shape) for i, shape in enumerate([(8, 2, 64), (8, 4, 128), (3, 3, 32), (16, 1, 64), (4, 2, 128)])]
+    data = [(*inputs(lengths, h, hk, d, BF16, seed=i), cu_of(lengths)) for i, (lengths, h, hk, d) in enumerate(sets)]
+    want = []
+    for q, k, v, do, cu in data:
+        want.append(run(q, k, v, cu, do))
+        torch.cuda.synchronize()
+    for _ in range(6):
+        got = [run(q, k, v, cu, do) for q, k, v, do, cu in data * 3]
+        for i, g in enumerate(got):
+            assert all(torch.equal(g[n], want[i % len(data)][n]) for n in g), i
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [run(q, k, v, cu, do) for q, k, v, do, cu in data * 2]
+    for _ in range(5):
+        for g in got:
+            for t in g.values():
+                t.zero_()
+        graph.replay()
+        for i, g in enumerate(got):
+            assert all(torch.equal(g[n], want[i % len(data)][n]) for n in g), i
+
+
+def test_offsets_beyond_32_bits():
+    """2.3e9 elements in q and its gradient."""
+    lengths, heads, d = [128] * 4400 + [77], 32, 128
+    rows = sum(lengths)
+    q, do = (torch.randn(rows, heads, d, device="cuda", dtype=BF16) for _ in range(2))
+    k, v = (torch.randn(rows, 1, d, device="cuda", dtype=BF16) for _ in range(2))
+    got = run(q, k, v, cu_of(lengths), do)
+    for first, of in ((0, lengths[:2]), (rows - 205, lengths[-2:])):
+        part = slice(first, first + sum(of))
+        for name, (value, tolerance) in exact_packed(*(t[part] for t in (q, k, v)), of, do[part], None).items():
+            assert ((got[name][part].double() - value).abs() <= tolerance).all(), (name, first)
