@@ -17,8 +17,8 @@
 // movmatrix.  Eight query heads fill the product; as its rows they would fill half of it.  The four warps meet
 // where a (sequence, key head) ends, while their next stages are already loading.  The products take a fraction of
 // the time that the bytes take, so mma.sync serves, and a row of eight queries needs no tile of 128.
-// 128 sequences of 500 to 8192 keys (344 905 in all), 32 / 8 heads of 128 columns, pages of 16: 237 us, 91 % of the measured copy
-// rate.  Two sequences of 100 000 to 131 072, 16 / 2 heads of 128, pages of 64: 56 us, 50 of them decode_kernel (5.3 TB/s).
+// 128 sequences of 500 to 8192 keys (344 905 in all), 32 / 8 heads of 128 columns, pages of 16: 233 us, 92 % of the measured copy
+// rate.  Two sequences of 100 000 to 131 072, 16 / 2 heads of 128, pages of 64: 53.5 us, 47 of them decode_kernel (5.6 TB/s).
 #include <algorithm>
 
 #include "common.cuh"
@@ -549,7 +549,10 @@ __global__ void __launch_bounds__(kJoinMost) decode_join_kernel(const __grid_con
                                                                 int slots, int ctas) {
   __shared__ float4 shared[kJoinMost];  // sums of two columns, maximum, sum of the weights
   grid_wait_previous();
-  grid_allow_next();
+  // No grid_allow_next: CTAs of the next decode_kernel that start under this one find its small blocks of shared memory taken in the middle
+  // of an SM's and settle around them; what these leave behind is in two pieces, too small for the SM's last CTA, which then
+  // runs after the others (64 sequences of 204 000 keys, 12 heads of 64 columns: 170 us against 134).  So it starts when the last CTA
+  // here has ended, which is 2 us earlier than an ordinary launch (two of 131 072 keys: 56 -> 53.5, 345 000 keys in 128: 237 -> 233).
   const Workspace space(a.workspace, slots, ctas);
   const int place_rows = hp * rows, row = blockIdx.x % place_rows;
   const uint4 c = ld_global(reinterpret_cast<const uint4*>(space.cuts) + blockIdx.x / place_rows);
@@ -631,16 +634,7 @@ cudaError_t launch_decode_s(const CUtensorMap& tk, const CUtensorMap& tv, const 
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   const DecodeGrid g = decode_grid(a.batch, a.Hq, a.Hkv, a.D, a.table_width, a.page_size, std::min(num_sms * C::kCtasPerSm, kMaxCtas));
-  // With more than one CTA to an SM an ordinary launch.  CTAs that start under the end of the kernel before find small blocks
-  // of shared memory taken in the middle of an SM's and settle around them; what these leave behind is in two pieces, too small
-  // for the SM's last CTA, which then runs after the others (64 sequences of 204 000 keys, 12 heads of 64 columns:
-  // 170 us against 134).  Single CTAs gain the 1.5 us that the early start is worth.
-  if (g.ctas <= num_sms) {
-    e = launch_dependent(kern, g.ctas, 32 * kWarps, C::kSmemBytes, stream, tk, tv, a, g.rows, g.cuts, box_rows, status);
-  } else {
-    kern<<<g.ctas, 32 * kWarps, C::kSmemBytes, stream>>>(tk, tv, a, g.rows, g.cuts, box_rows, status);
-    e = cudaGetLastError();
-  }
+  e = launch_dependent(kern, g.ctas, 32 * kWarps, C::kSmemBytes, stream, tk, tv, a, g.rows, g.cuts, box_rows, status);
   if (e != cudaSuccess) return e;
   // as many shares as take the parts of a cut at once, were the cuts alike
   const int batches = (g.ctas / g.cuts + kJoinBatch) / kJoinBatch;

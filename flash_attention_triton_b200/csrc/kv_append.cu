@@ -97,8 +97,7 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
   __shared__ TokenPlace places[kMaxTokens];
   const int first = blockIdx.x / slices * tokens_per_cta, slice = blockIdx.x % slices;
   const int count = min(tokens_per_cta, a.tokens - first);
-  grid_wait_previous();
-  grid_allow_next();
+  grid_wait_previous();  // and no grid_allow_next, for the reason at decode_join_kernel
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, row = first + lane;
     int sequence = row, fresh = 1, index = 0, length = 0;
