@@ -97,7 +97,9 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   if (int e = launch_context(&ctx)) return e;
   const PackedShape s = make_shape(rows, batch, Hq, Hkv, D, dtype, scale);
   const PackedPlan p = packed_plan(const_cast<void*>(plan), rows, batch);
-  const PackedStats stats{static_cast<float*>(workspace), static_cast<unsigned*>(workspace) + static_cast<size_t>(p.capacity) * Hq * 256};
+  unsigned* const words = static_cast<unsigned*>(workspace);
+  const size_t heads = static_cast<size_t>(p.capacity) * Hq;
+  const PackedStats stats{static_cast<float*>(workspace), words + heads * 256, words + heads * (256 + 4)};
   const int cluster = packed_cluster(s, ctx.num_sms);
   const int step = packed_step_rows(s, Hkv * cluster, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
   CUtensorMap tq, tk, tv, tdo, tdq, tdk, tdv;

@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
   __shared__ unsigned amax[kPreHeads];
   grid_wait_previous();
   grid_allow_next();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *out.written = 0;
   const int parts = 4 * ((Hq + kPreHeads - 1) / kPreHeads);  // CTAs of a tile
   const int entry = blockIdx.x / parts, part = blockIdx.x - entry * parts;
   // (asked for together: an entry behind the last one may hold anything)

@@ -54,9 +54,10 @@ struct PackedShape {
 struct PackedStats {
   float* stats;
   unsigned* amax;
+  unsigned* written;  // zero behind the preprocess; 1 once the dK / dV kernel has seen it complete
 };
 inline size_t packed_stats_bytes(int rows, int batch, int Hq) {
-  return static_cast<size_t>(packed_capacity(rows, batch)) * Hq * (256 + 4) * 4;
+  return static_cast<size_t>(packed_capacity(rows, batch)) * Hq * (256 + 4) * 4 + 16;
 }
 
 // Status word of cu_seqlens that fall, or leave the rows: every output is zero then.

@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
   const uint32_t tmem_base = *tmem_slot;
   const WaitCtx w{abort_flag, status};
   grid_wait_previous();
+  if (blockIdx.x == 0 && threadIdx.x == 0) release_flag(stats.written);
   grid_allow_next();
 
   static_assert(S == 1 || S == 2 || S == 4, "packed_cluster");
@@ -377,8 +378,8 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
 // =========================================================================================
 // dQ: one CTA per Q tile of a query head, KV tiles in ascending order
 // =========================================================================================
-// It needs nothing of the dK / dV kernel in front of it, so its CTAs work as soon as they find room, under that one's
-// last CTAs.  fp16, eight sequences of 256 to 1024 rows, 16 / 4 heads of 64 columns, whole training pass: 101.6 us when they wait, 89.1;
+// It needs nothing of the dK / dV kernel in front of it, which reads no output, so its CTAs work as soon as they find room, under
+// that one's last CTAs (a kernel for both needs one CTA to an SM for dQ as well: 99.2).  fp16, eight sequences of 256 to 1024 rows, 16 / 4 heads of 64 columns, whole training pass: 101.6 us when they wait, 89.1;
 // 4096 rows, backward alone 163 and 155.
 template <int D, int W>
 struct PackedDqCfg {
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(PackedDqCfg<D, W>::kThreads, PackedDqCfg<D, W>
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const WaitCtx w{abort_flag, status};
-  grid_acquire_earlier();  // the dK / dV kernel in front leaves nothing for this one
+  grid_wait_unless(stats.written);
   grid_allow_next();
 
   const int entry = blockIdx.x / Hq, head = blockIdx.x - entry * Hq;

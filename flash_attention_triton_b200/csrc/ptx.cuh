@@ -123,10 +123,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, co
 // ----------------------------------------------------------------------------------------
 __device__ __forceinline__ void grid_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-// In place of grid_wait_previous for a kernel that reads and writes nothing of its predecessor's, only of the kernels before that
-// one, which have completed when it starts: what they wrote is seen from here on.  One CTA of it must wait for the predecessor before it
-// ends, so that the kernel does not complete before it.
-__device__ __forceinline__ void grid_acquire_earlier() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+// For a kernel that touches nothing its predecessor reads or writes, only what kernels before that one have left.  The predecessor
+// releases a flag behind its own wait, and who acquires it has seen all that the predecessor's wait made visible, the
+// asynchronous copies' view included; without the flag (zeroed by a kernel before) the wait is the usual one.  One CTA must wait
+// for the predecessor before it ends, so that the kernel does not complete before it.
+__device__ __forceinline__ void release_flag(unsigned* flag) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+}
+__device__ __forceinline__ void grid_wait_unless(const unsigned* flag) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+  if (v != 1u) grid_wait_previous();
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
 
 // Loads of what an earlier kernel of the stream wrote, which may still be running when this one starts.  The
 // read-only path (__ldg, ld.global.nc, what the compiler makes of a const __restrict__ parameter) is for

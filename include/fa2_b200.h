@@ -272,6 +272,7 @@ int fa2_bwd_static_scratch(const void* q, const void* k, const void* v, const vo
  * fa2_packed_bwd recomputes the scores for dK / dV and for dQ, so it needs no memory beyond O(rows): `workspace`
  * (16-byte aligned, fa2_packed_bwd_workspace_bytes) holds the row statistics.  dk and dv are summed over the query heads
  * of a key head in 32 bits; every sum has one owner and one order, so the same call gives the same bits.
+ * dq, dk and dv overlap none of the inputs, the plan or the workspace: their kernels run side by side.
  * strides (elements, row and head of each): q, k, v (6 values), backward q, k, v, dout (8 values); NULL: dense.  o, dq, dk, dv are dense.
  */
 size_t fa2_packed_plan_bytes(int rows, int batch);

@@ -70,7 +70,7 @@ def test_sizes():
     lib = _lib.lib()
     tiles = 1000 // 128 + 3  # at most, of 1000 rows in 3 sequences
     assert lib.fa2_packed_plan_bytes(1000, 3) == 16 + 2 * 16 * tiles
-    assert lib.fa2_packed_bwd_workspace_bytes(1000, 3, 4) == tiles * 4 * (256 + 4) * 4
+    assert lib.fa2_packed_bwd_workspace_bytes(1000, 3, 4) == tiles * 4 * (256 + 4) * 4 + 16
     assert lib.fa2_packed_plan_bytes(-1, 3) == lib.fa2_packed_plan_bytes(10, 0) == 0
 
 

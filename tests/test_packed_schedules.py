@@ -25,7 +25,8 @@ inline int __popc(unsigned x) { return __builtin_popcount(x); }
 namespace fa2 {
 inline uint32_t cluster_address(uint32_t a, uint32_t) { return a; }
 FA2_NOTHING(cluster_sync) FA2_NOTHING(st_cluster_v4)
-inline void grid_acquire_earlier() { sim_wait_previous(); }
+inline void grid_wait_unless(const unsigned*) { sim_wait_previous(); }
+FA2_NOTHING(release_flag)
 }
 """
 
