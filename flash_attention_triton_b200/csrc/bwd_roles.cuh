@@ -141,26 +141,29 @@ __device__ __forceinline__ void store_rows_f32(uint32_t tmem_row_addr, const F32
 // form dS * 2^k with the power of two that brings the largest |dO| of the (batch, head) problem
 // into [1, 2) and multiply the dK and dQ accumulators, which are linear in dS, by 2^-k before
 // the final rounding: exact, as long as nothing leaves the 16-bit range, and independent of how the
-// (batch, head) problems are partitioned.  `tile_amax` holds, per Q tile of the head, the largest
-// |dO| as its 16-bit pattern with the sign cleared (written by the preprocess kernel); called by
-// a whole warp.  Returns 2^k and stores 2^-k in *inverse; 1 for an all-zero or non-finite head.
+// (batch, head) problems are partitioned.  `most` is the largest |dO| as its 16-bit pattern with the
+// sign cleared.  Returns 2^k and stores 2^-k in *inverse; 1 for an all-zero or non-finite head.
+template <bool BF16>
+__device__ __forceinline__ float dscale_of(unsigned most, float* inverse) {
+  int k = 0;
+  if constexpr (BF16) {
+    const int e = static_cast<int>((most >> 7) & 0xffu);  // biased by 127
+    if (e != 0 && e != 255) k = 127 - e;
+  } else {
+    const int e = static_cast<int>((most >> 10) & 0x1fu);  // biased by 15
+    if (e != 31 && most != 0) k = 15 - (e == 0 ? 1 : e);   // subnormal: the smallest normal exponent
+  }
+  k = k < -100 ? -100 : (k > 100 ? 100 : k);
+  *inverse = __uint_as_float(static_cast<unsigned>(127 - k) << 23);
+  return __uint_as_float(static_cast<unsigned>(127 + k) << 23);
+}
+// From `tile_amax`, the largest |dO| of each Q tile of the head (written by the preprocess kernel); called by a whole warp.
 template <bool BF16>
 __device__ __forceinline__ float head_dscale(const unsigned* tile_amax, int ntiles,
                                              int lane, float* inverse) {
   unsigned m = 0;
   for (int t = lane; t < ntiles; t += 32) m = max(m, ld_global(tile_amax + t));
-  m = __reduce_max_sync(0xffffffffu, m);
-  int k = 0;
-  if constexpr (BF16) {
-    const int e = static_cast<int>((m >> 7) & 0xffu);  // biased by 127
-    if (e != 0 && e != 255) k = 127 - e;
-  } else {
-    const int e = static_cast<int>((m >> 10) & 0x1fu);  // biased by 15
-    if (e != 31 && m != 0) k = 15 - (e == 0 ? 1 : e);   // subnormal: the smallest normal exponent
-  }
-  k = k < -100 ? -100 : (k > 100 ? 100 : k);
-  *inverse = __uint_as_float(static_cast<unsigned>(127 - k) << 23);
-  return __uint_as_float(static_cast<unsigned>(127 + k) << 23);
+  return dscale_of<BF16>(__reduce_max_sync(0xffffffffu, m), inverse);
 }
 
 // Number of (KV tile, Q tile) pairs of one head whose KV tile index is below `jt`, with

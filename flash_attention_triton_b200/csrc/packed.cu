@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
   const int quarter = part & 3, h0 = part / 4 * kPreHeads, heads = min(Hq - h0, kPreHeads);
   const int local = e.tile * 128 + quarter * 32;  // first of the 32 rows in the sequence
   const int here = min(max(e.length - local, 0), 32);
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, G = Hq / Hkv;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   if (threadIdx.x < kPreHeads) amax[threadIdx.x] = 0;
   // the result that this thread writes at the end
   static_assert(kPreHeads * 32 == kPreThreads, "one result a thread");
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kPreThreads) packed_preprocess_kernel(
   to[0] = inside ? -row_lse * kLog2e : -INFINITY;
   to[128] = inside ? -delta[out_h][out_r] : 0.f;
   if (!BF16 && out_r == 0)
-    out.amax[((static_cast<size_t>(h / G) * capacity + e.base + e.tile) * 4 + quarter) * G + h % G] = amax[out_h];
+    out.amax[(static_cast<size_t>(h) * capacity + e.base + e.tile) * 4 + quarter] = amax[out_h];
 }
 
 }  // namespace

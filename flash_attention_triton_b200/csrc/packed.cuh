@@ -50,7 +50,7 @@ struct PackedShape {
 };
 
 // What the backward's preprocess leaves: -lse log2(e) and -delta by tile, [Hq][capacity][2][128], rows behind a
-// sequence -inf and 0; at fp16 also the largest |dout| of every 32 rows, [Hkv][capacity][4][G] (see head_dscale).
+// sequence -inf and 0; at fp16 also the largest |dout| of every 32 rows, [Hq][capacity][4] (see head_dscale).
 struct PackedStats {
   float* stats;
   unsigned* amax;

@@ -64,16 +64,23 @@ __device__ __forceinline__ void store_packed_rows(uint32_t tmem_row_addr, uint8_
   }
 }
 
-// The power of two that dS carries at fp16 (head_dscale), common to the query heads of a key head because their
-// products meet in one accumulator; bf16 has the exponents of fp32 and needs none.
+// The power of two that dS carries at fp16 (head_dscale), by the largest |dO| of `heads` query heads from `head` on.  For dQ that is
+// the one head of the product; for dK and dV all of a key head, because their products meet in one accumulator.  bf16 has the
+// exponents of fp32 and needs none.
 template <bool BF16>
-__device__ __forceinline__ float group_dscale(const PackedStats& stats, int capacity, int base, int tiles, int kv_head, int G,
+__device__ __forceinline__ float heads_dscale(const PackedStats& stats, int capacity, int base, int tiles, int head, int heads,
                                               int lane, float* inverse) {
   if constexpr (BF16) {
     *inverse = 1.f;
     return 1.f;
   } else {
-    return head_dscale<false>(stats.amax + (static_cast<size_t>(kv_head) * capacity + base) * 4 * G, tiles * 4 * G, lane, inverse);
+    const int words = 4 * tiles;  // of a head, one behind the other
+    unsigned m = 0;
+    for (int i = lane; i < heads * words; i += 32) {
+      const int h = i / words;
+      m = max(m, ld_global(stats.amax + (static_cast<size_t>(head + h) * capacity + base) * 4 + (i - h * words)));
+    }
+    return dscale_of<false>(__reduce_max_sync(0xffffffffu, m), inverse);
   }
 }
 
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
     const uint32_t tDpt = tmem_base + lane_base + C::kColDpt + wg * kCols;
     const float2 sc2 = make_float2(scale_log2, scale_log2);
     float inv_dscale;
-    const float dscale = group_dscale<BF16>(stats, capacity, e.base, ntiles, kv_head, G, lane, &inv_dscale);
+    const float dscale = heads_dscale<BF16>(stats, capacity, e.base, ntiles, kv_head * G, G, lane, &inv_dscale);
     const float2 scale2 = make_float2(scale * dscale, scale * dscale);  // dS = P (dP - delta) scale 2^k
     bool ok = true;
     for (int t = 0, u = 0; t < nsteps; ++t, u = u + 1 == per_head ? 0 : u + 1) {
@@ -591,7 +598,7 @@ __global__ void __launch_bounds__(PackedDqCfg<D, W>::kThreads, PackedDqCfg<D, W>
     const uint32_t tDp = tmem_base + lane_base + C::kColDp + wg * kCols;
     const float2 sc2 = make_float2(scale_log2, scale_log2);
     float inv_dscale;
-    const float dscale = group_dscale<BF16>(stats, capacity, e.base, (e.length + 127) >> 7, hk.h, G, lane, &inv_dscale);
+    const float dscale = heads_dscale<BF16>(stats, capacity, e.base, (e.length + 127) >> 7, head, 1, lane, &inv_dscale);
     const float2 scale2 = make_float2(scale * dscale, scale * dscale);
     bool ok = mbar_wait_warp(bar(C::kBarQ), 0, w, kBSiteCmpQ);
     float2 nlse2 = make_float2(0.f, 0.f), ndlt2 = make_float2(0.f, 0.f);
