@@ -42,6 +42,16 @@ __host__ __device__ __forceinline__ uint32_t swizzled_offset_128B(uint32_t row, 
   return off ^ (((off >> 7) & 7u) << 4);
 }
 
+// A forward's weights enter the second product in 16 bits.  fp16 keeps nothing below 2^-25, and where nearly all of a row's weight
+// lies on one key whose values are small, thousands of weights below that can be the result: 8 192 keys 17.5 nats under the one have
+// 2.1e-4 of the weight.  So fp16 weights are formed as P 2^11, which cancels against their sum: in a row whose largest
+// weight is 1 they keep all bits down to 2^-25 and are off by 2^-36 at most below.  fp16 ends at 2^16, which leaves 2^4 for how far the
+// running maximum may lag behind.  bf16 has the exponents of fp32.
+template <bool BF16>
+constexpr float kWeightPower = BF16 ? 0.0f : 11.0f;  // logarithm to 2
+template <bool BF16>
+constexpr float weight_lag(float lag) { return BF16 || lag < 4.0f ? lag : 4.0f; }  // the same, of the largest factor above the running maximum
+
 // ----------------------------------------------------------------------------------------
 // Host launchers (one per kernel family), defined in the .cu files of this directory.
 // Tensor maps describe [B, H, N, D] tensors with box (CH, 128, 64 or 32, 1, 1).

@@ -57,7 +57,8 @@ struct FwdCfg {
   // O is rescaled when the running maximum has moved by more than this (log2 units).  A row's
   // largest P is exactly 1, without rounding error, when its maximum is fresh: 64-row tiles, whose
   // maxima settle later, use a lower threshold and none after their first tile, which keeps the
-  // error of O below that of 128-row tiles (peaked softmax, fp16: 1.78e-4 against 1.84e-4).
+  // error of O below that of 128-row tiles (peaked softmax, fp16: 1.78e-4 against 1.84e-4).  At fp16 no tile takes more
+  // than 4, for the room that P 2^11 needs (weight_lag): [2,16,8192,64] fp16 336 us with 8 and 330 to 337 with 4.
   static constexpr float kRescaleThreshold = kW == 64 ? 4.0f : 8.0f;
   static constexpr int kKvBytes = T::kTileBytes / 128 * kW;
   // registers of a producer / softmax thread; the launch gives every thread
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdCfg<D == 256 ? 128 : D, W>::kC
       }
       float m_new = max3(m_run, mx[0], mx[1]);
       if constexpr (W == 128) m_new = fmaxf(m_new, fmaxf(mx[2], mx[3]));
-      const float threshold = W == 128 ? C::kRescaleThreshold : (j == 1 ? 0.f : C::kRescaleThreshold);
+      const float threshold = W == 64 && j == 1 ? 0.f : weight_lag<BF16>(C::kRescaleThreshold);
       const bool need = (m_new - m_run) * scale_log2 > threshold;
       bool pv_waited = false;
       if (__any_sync(0xffffffffu, need)) {
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdCfg<D == 256 ? 128 : D, W>::kC
       const float2 sc2 = make_float2(scale_log2, scale_log2);
       // A row whose scores so far are all -inf (infinite inputs, or finite ones whose product overflows) has
       // weights 0 (2^-126 from the polynomial) and not -inf + inf; its first finite score rescales them away.
-      const float neg_m = m_run == -INFINITY ? 0.f : -m_run * scale_log2;
+      const float neg_m = m_run == -INFINITY ? 0.f : kWeightPower<BF16> - m_run * scale_log2;
       const float2 nm2 = make_float2(neg_m, neg_m);
       float2 acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
       uint32_t pk[W / 2];
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdCfg<D == 256 ? 128 : D, W>::kC
       }
       tc_fence_before();  // O_i is overwritten by the next item's first product, which this group's P lets in
       if (row < N)
-        lse[static_cast<size_t>(item.bh) * N + row] = (m_run * scale_log2 + lg2(l_run)) * kLn2;
+        lse[static_cast<size_t>(item.bh) * N + row] = (m_run * scale_log2 + (lg2(l_run) - kWeightPower<BF16>)) * kLn2;
     }
     if constexpr (C::kStageInQ) {
       // A group without a tile has waited for nothing yet: its arrival must not count for the item before.

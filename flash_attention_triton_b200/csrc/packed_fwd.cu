@@ -23,7 +23,7 @@ template <int D>
 struct PackedFwdCfg {
   using T = Tile<D>;
   static constexpr int kPolyShare = D == 32 ? 3 : 0;  // as FwdCfg
-  static constexpr float kRescaleThreshold = 8.0f;
+  static constexpr float kRescaleThreshold = 8.0f;  // as FwdCfg: 4 at fp16
   static constexpr int kLaunchRegs = 65536 / kThreads / 8 * 8;
   static constexpr int kProducerRegs = 72;
   static constexpr int kSoftmaxRegs = 216;
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int local = qt * 128 + (warp & 3) * 32;  // first row of this warp in the sequence
       const bool mine = local + lane < item.length;
       // rows behind the sequence ask for no rescale, so that what they hold changes no bit of the others
-      const float threshold = mine ? C::kRescaleThreshold : INFINITY;
+      const float threshold = mine ? weight_lag<BF16>(C::kRescaleThreshold) : INFINITY;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < nj; ++j) {
         const int ph = (done + j) & 1;  // of this tile on the group's barriers
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // p = 2^(s*c - m*c) with packed fp32x2 FMAs; row sum in four independent packed chains
         const float2 sc2 = make_float2(scale_log2, scale_log2);
         // a row whose scores so far are all -inf has weights 0; its first finite score rescales them away
-        const float neg_m = m_run == -INFINITY ? 0.f : -m_run * scale_log2;
+        const float neg_m = m_run == -INFINITY ? 0.f : kWeightPower<BF16> - m_run * scale_log2;
         const float2 nm2 = make_float2(neg_m, neg_m);
         float2 acc[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
         uint32_t pk[64];
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tc_fence_before();  // O_i is overwritten by the next item's first product, which this group's P lets in
-        if (mine) lse[static_cast<size_t>(head) * rows + row] = (m_run * scale_log2 + lg2(l_run)) * kLn2;
+        if (mine) lse[static_cast<size_t>(head) * rows + row] = (m_run * scale_log2 + (lg2(l_run) - kWeightPower<BF16>)) * kLn2;
       }
     }  // items
     if (lane == 0) tma_store_wait_read();
