@@ -49,7 +49,15 @@ struct PackedShape {
   float scale;
 };
 
-// What the backward's preprocess leaves: -lse log2(e) and -delta by tile, [Hq][capacity][2][128], rows behind a
+// The backward's P, from lse and at most 1, carries this power of two at fp16 for the reason at kWeightPower (common.cuh): a key whose
+// weights are small in thousands of rows has its dV from them.  It comes with the exponent, and dV and dS give it back: off by 2^-39 at
+// most below 2^-28.  2^16, where fp16 ends, leaves 2^2 for the rounding of lse beside scores of millions.
+template <bool BF16>
+constexpr float kProbabilityPower = BF16 ? 0.0f : 14.0f;  // logarithm to 2
+template <bool BF16>
+constexpr float kProbabilityInverse = BF16 ? 1.0f : 1.0f / 16384;
+
+// What the backward's preprocess leaves: -lse log2(e) + kProbabilityPower and -delta by tile, [Hq][capacity][2][128], rows behind a
 // sequence -inf and 0; at fp16 also the largest |dout| of every 32 rows, [Hq][capacity][4] (see head_dscale).
 struct PackedStats {
   float* stats;

@@ -285,13 +285,14 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
     const float2 sc2 = make_float2(scale_log2, scale_log2);
     float inv_dscale;
     const float dscale = heads_dscale<BF16>(stats, capacity, e.base, ntiles, kv_head * G, G, lane, &inv_dscale);
-    const float2 scale2 = make_float2(scale * dscale, scale * dscale);  // dS = P (dP - delta) scale 2^k
+    const float ds_scale = scale * dscale * kProbabilityInverse<BF16>;  // dS = P (dP - delta) scale 2^k
+    const float2 scale2 = make_float2(ds_scale, ds_scale);
     bool ok = true;
     for (int t = 0, u = 0; t < nsteps; ++t, u = u + 1 == per_head ? 0 : u + 1) {
       const int s = t % C::kStages, ph = (t / C::kStages) & 1;
       const int row = q_row(u), qt = row >> 7;
       const float* st = reinterpret_cast<const float*>(smem + C::kOffStats + s * (W * 8));
-      const float4* nlse = reinterpret_cast<const float4*>(st + wg * kCols);      // -lse*log2e
+      const float4* nlse = reinterpret_cast<const float4*>(st + wg * kCols);      // -lse*log2e (+ kProbabilityPower)
       const float4* ndlt = reinterpret_cast<const float4*>(st + W + wg * kCols);  // -delta
       if (!(ok = mbar_wait_warp(bar(C::kBarQFull + s), ph, w, kBSiteCmpQ))) break;
       if (!(ok = mbar_wait_warp(bar(C::kBarStFull + t % C::kStBars), (t / C::kStBars) & 1, w, kBSiteCmpSt))) break;
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(DkdvCfg<D, 0, W>::kThreads, DkdvCfg<D, 0, W>::
     }
     if (ok && owner == rank)
       store_packed_rows<D, BF16, KD>(sums, smem + (wg == 0 ? C::kOffV : C::kOffK), w4, lane, wg == 0 ? &tdv : &tdk, row_k + w4 * 32,
-                                     kv_head, Hkv, left - w4 * 32, wg == 0 ? dv : dk, cols, wg == 0 ? 1.0f : inv_dscale,
+                                     kv_head, Hkv, left - w4 * 32, wg == 0 ? dv : dk, cols, wg == 0 ? kProbabilityInverse<BF16> : inv_dscale,
                                      reinterpret_cast<const float*>(smem + C::kOffQ) + at, S - 1, kSenderFloats);
   }
   }
@@ -599,12 +600,13 @@ __global__ void __launch_bounds__(PackedDqCfg<D, W>::kThreads, PackedDqCfg<D, W>
     const float2 sc2 = make_float2(scale_log2, scale_log2);
     float inv_dscale;
     const float dscale = heads_dscale<BF16>(stats, capacity, e.base, (e.length + 127) >> 7, head, 1, lane, &inv_dscale);
-    const float2 scale2 = make_float2(scale * dscale, scale * dscale);
+    const float ds_scale = scale * dscale * kProbabilityInverse<BF16>;
+    const float2 scale2 = make_float2(ds_scale, ds_scale);
     bool ok = mbar_wait_warp(bar(C::kBarQ), 0, w, kBSiteCmpQ);
     float2 nlse2 = make_float2(0.f, 0.f), ndlt2 = make_float2(0.f, 0.f);
     if (ok) {
       const float* st = reinterpret_cast<const float*>(smem + C::kOffStats);
-      nlse2 = make_float2(st[r], st[r]);              // -lse*log2e of this row
+      nlse2 = make_float2(st[r], st[r]);              // -lse*log2e of this row (+ kProbabilityPower)
       ndlt2 = make_float2(st[128 + r], st[128 + r]);  // -delta of this row
     }
     for (int j = 0; ok && j < nkv; ++j) {

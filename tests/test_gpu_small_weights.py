@@ -97,3 +97,23 @@ def test_the_largest_weights_come_late():
     for h in range(2):
         check(o[:, h], q[:, h], k[:, 0], v[:, 0])
         check(dense[0, h], q[:, h], k[:, 0], v[:, 0])
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,d", [(8192, 2, 1, 64), (4096, 4, 1, 128), (8192, 1, 1, 32)])
+def test_packed_value_gradient(n, heads, kv_heads, d):
+    """dV of a key is its column of weights times dO: P comes from lse, at most 1, and carries 2^14, so
+    below the normal numbers it is off by 2^-39."""
+    q, k, v, do = rows(n, heads, kv_heads, d, FP16)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dv = torch.autograd.grad(flash_attention_packed(*leaves, cu, SCALE), leaves, do)[2]
+    q, k, v = (t.detach() for t in leaves)
+    for j in range(kv_heads):
+        want, group = torch.zeros(n, d, dtype=torch.float64, device="cuda"), heads // kv_heads
+        for h in range(j * group, (j + 1) * group):
+            want += exact(q[:, h], k[:, j], v[:, j])[2].T @ do[:, h].double()
+        e = (d + 8) * 2.0**-24 * 20 + 1e-4
+        # (dO is positive, so the sum of magnitudes is the result)
+        tolerance = 2.0**-11 * want + (2.0**-11 + 2 * e + group * n * 2.0**-24) * want + 2.0**-39 * group * n * do.max().item() + 2.0**-25
+        off = (dv[:, j].double() - want).abs()
+        assert (off <= tolerance).all(), ((off / tolerance).max().item(), off.max().item())
