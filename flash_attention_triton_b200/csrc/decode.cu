@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
   uint32_t qb[HP][kSteps][NT][2];
   float o[HP][kSteps][NT][4];  // rows (columns of V) 16 i + lane / 4 (+ 8), columns (query heads) 8 t + 2 (lane % 4) (+ 1)
   float m[HP][NT][2], l[HP][NT][2];
-  const float threshold = 8.f / a.scale_log2;
+  const float threshold = weight_lag<BF16>(8.f) / a.scale_log2;
   uint32_t phases = 0;  // bit s: parity of the next wait on stage s
   bool fresh = true, ok = true;
   bool begins = work.unit == 0;  // the first unit of the (sequence, key head) is in this stretch
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
             need |= fmaxf(s[p][t][e], s[p][t][2 + e]) - m[p][t][e] > threshold;
           }
       }
-      // The maximum follows only when a score is 2^8 above it: a weight is at most 2^8 then.
+      // The maximum follows only when a score is 2^8 (fp16: 2^4) above it: a weight is at most 2^8 (P 2^11 at fp16: 2^15) then.
       if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
         for (int p = 0; p < HP; ++p)
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
               for (int i = 0; i < kSteps; ++i) o[p][i][t][e] *= alpha, o[p][i][t][2 + e] *= alpha;
             }
       }
-      // P^T in 16 bits; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
+      // P^T in 16 bits, with kWeightPower, which cancels in the end; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
       // term is p (1 - 2^-8) rounded, at most p (1 - 2^-16), so that the second one is positive where p is, and an
       // infinite value stays infinite in both products.
       // V^T: the 16 x 16 piece of V is turned around on its way, so the lanes' rows and halves change places.
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float shift = m[p][t][e] == -INFINITY ? 0.f : -m[p][t][e] * a.scale_log2;
+            const float shift = m[p][t][e] == -INFINITY ? 0.f : kWeightPower<BF16> - m[p][t][e] * a.scale_log2;
             s[p][t][e] = ex2(fmaf(s[p][t][e], a.scale_log2, shift));
             s[p][t][2 + e] = ex2(fmaf(s[p][t][2 + e], a.scale_log2, shift));
             l[p][t][e] += s[p][t][e] + s[p][t][2 + e];

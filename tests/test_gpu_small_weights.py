@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from flash_attention_triton_b200 import _lib, flash_attention_packed, flash_attention_v2
+from paged_helpers import Cache, fa
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -117,3 +118,22 @@ def test_packed_value_gradient(n, heads, kv_heads, d):
         tolerance = 2.0**-11 * want + (2.0**-11 + 2 * e + group * n * 2.0**-24) * want + 2.0**-39 * group * n * do.max().item() + 2.0**-25
         off = (dv[:, j].double() - want).abs()
         assert (off <= tolerance).all(), ((off / tolerance).max().item(), off.max().item())
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("held,heads,kv_heads,d,page", [([2048] * 400, 3, 1, 64, 16), ([131072], 2, 1, 64, 64), ([8192, 2048] * 40, 4, 2, 128, 16),
+                                                        ([4096] * 80, 16, 1, 256, 32), ([1500] * 200, 4, 4, 40, 24), ([900] * 90, 2, 1, 64, 1)])
+def test_decode(held, heads, kv_heads, d, page, dtype):
+    """Here a warp loses the share of its own keys only, where it holds the one above the others."""
+    n = max(held)
+    q, k, v, _ = rows(n, heads, kv_heads, d, dtype, queries=len(held))
+    cache = Cache([0] * len(held), held, page, kv_heads, d, dtype)
+    for s, count in enumerate(held):
+        at = cache.places(s, range(count))
+        cache.k[at], cache.v[at] = k[:count], v[:count]
+    o = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths(held), SCALE)
+    for count in set(held):
+        s = [i for i, x in enumerate(held) if x == count]
+        for h in range(heads):
+            j = h * kv_heads // heads
+            check(o[s, h], q[s, h], k[:count, j], v[:count, j], causal=False)
