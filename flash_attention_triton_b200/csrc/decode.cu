@@ -241,14 +241,18 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
 
   const Workspace space(a.workspace, slots, gridDim.x);
   const bool by_segment = static_cast<long long>(a.batch) * heads * blocks == slots;  // what a Cut belongs to
-  // sequences without keys
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
-    if (ld_global(a.lengths + b) <= 0) {
+  // sequences without keys, and those with more than the block table has room for (2^31 - 1: as many as that)
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    const int n = ld_global(a.lengths + b);
+    if (threadIdx.x == 0 && n != 0x7fffffff && n > static_cast<long long>(a.table_width) * a.page_size)
+      atomicCAS(status, 0, kStatusPage | kSiteDecode);
+    if (n <= 0) {
       for (int i = threadIdx.x; i < a.Hq * d8; i += 32 * kWarps)
         reinterpret_cast<uint4*>(a.out)[static_cast<long long>(b) * a.Hq * d8 + i] = make_uint4(0, 0, 0, 0);
       if (by_segment)
         for (int h = threadIdx.x; h < heads * blocks; h += 32 * kWarps) space.cuts[b * heads * blocks + h] = make_int4(0, 0, 0, -1);
     }
+  }
 
   const long long total = row_length(a, heads, lane);
   const long long u0 = stretch_start(total, stretch, stretches), u1 = stretch_start(total, stretch + 1, stretches);
@@ -424,7 +428,9 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
       }
       // P^T in 16 bits, with kWeightPower, which cancels in the end; at bf16, whose 8 bits would be the largest error of the output, as a sum of two.  The first
       // term is p (1 - 2^-8) rounded, at most p (1 - 2^-16), so that the second one is positive where p is, and an
-      // infinite value stays infinite in both products.
+      // infinite value stays infinite in both products.  At fp16 one term's 11 bits are those of the output: its error is 1.34 times
+      // that of its rounding alone (2.78e-4 against 2.08e-4 of its norm, 32 sequences of 100 to 2000, 12 heads of 64), and a second term took
+      // 20.1 -> 21.05 us there, 125.6 -> 133 on 64 of 500 to 8192, 32 / 2 heads of 256, 83.2 -> 90.7 on 64 / 2 of 128.
       // V^T: the 16 x 16 piece of V is turned around on its way, so the lanes' rows and halves change places.
       const int vrow = (lane & 7) + ((lane >> 4) << 3), vhalf = (lane >> 3) & 1;
 #pragma unroll

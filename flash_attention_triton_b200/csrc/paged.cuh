@@ -39,7 +39,7 @@ struct DecodeArgs {
   const void *k_cache, *v_cache;
   void* out;      // dense [batch, Hq, D]
   const int* block_table;
-  const int* lengths;  // [batch]: keys of a sequence; out is zero where there are none
+  const int* lengths;  // [batch]: keys of a sequence, 2^31 - 1: all that the block table has room for; out is zero where there are none
   float* workspace;    // partial results, decode_workspace_floats()
   RowStrides sq;
   CacheStrides sk_cache, sv_cache;

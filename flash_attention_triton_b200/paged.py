@@ -89,7 +89,8 @@ def flash_attention_decode(
         q: ``[batch, heads, headdim]``; query head ``h`` reads key head ``h * kv_heads // heads``.
         k_cache, v_cache: the cache, of the type of ``q``; head dims are multiples of 8 up to 256.
         block_table: int32 ``[batch, width]``.
-        lengths: int32 ``[batch]``; the output of a sequence without positions is zero.
+        lengths: int32 ``[batch]``; the output of a sequence without positions is zero.  ``2**31 - 1`` stands for as many as the
+            block table has room for; any other length beyond that counts as that many and sets the status word.
         softmax_scale: scaling factor (default and 0.0: ``1/sqrt(headdim)``).
 
     Returns:

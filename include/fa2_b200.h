@@ -318,7 +318,8 @@ int fa2_kv_append(const void* q, const void* k, const void* v, void* q_out, void
 
 /*
  * out[s, h] = softmax(scale * q[s, h] K^T) V over the first lengths[s] positions of sequence s, with the keys and values of
- * head h * Hkv / Hq; zeros where lengths[s] <= 0.  q [batch, Hq, D], out dense [batch, Hq, D].  The cache is cut over all SMs
+ * head h * Hkv / Hq; zeros where lengths[s] <= 0.  A length of 2^31 - 1 stands for as many positions as the block table has
+ * room for and sets no status; of any other length the positions beyond the block table are left out, as said above.  q [batch, Hq, D], out dense [batch, Hq, D].  The cache is cut over all SMs
  * whatever the lengths are; `workspace` (16-byte aligned, fa2_decode_workspace_bytes) holds the parts that are joined in
  * a fixed order, so the same call gives the same bits.
  * strides (elements): q (row, head), k_cache, v_cache (page, slot, head), block_table (row), 9 values; NULL: dense.

@@ -1,0 +1,55 @@
+"""flash_attention_decode at the edges of its arguments."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from flash_attention_triton_b200 import _lib
+from paged_helpers import Cache, fa
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _no_status():
+    yield
+    assert _lib.device_status() == 0
+
+
+def normal(*shape, dtype, seed=1):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("batch,late", [(1, 0), (3, 1), (700, 699)])
+def test_a_length_beyond_the_block_table_sets_the_status(batch, late, page):
+    """The keys that have a place count; the status word says that there are others."""
+    held = [5 * page] * batch
+    cache = Cache(held, held, page, 2, 64, BF16)
+    q = normal(batch, 4, 64, dtype=BF16)
+    clean = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
+    assert _lib.device_status() == 0
+    for more in (1, 1000, 2**31 - 2 - 5 * page):
+        lengths = cache.lengths()
+        lengths[late] += more
+        out = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, lengths)
+        assert _lib.device_status() == 0x40002
+        assert torch.equal(out, clean)
+
+
+def test_a_length_beyond_the_block_table_raises_where_asked(monkeypatch):
+    cache = Cache([64], [64], 16, 2, 64, BF16)
+    q = normal(1, 4, 64, dtype=BF16)
+    monkeypatch.setenv("FA2_B200_CHECK_STATUS", "1")
+    fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths([64]))
+    with pytest.raises(_lib.Fa2Error, match="outside the cache"):
+        fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths([65]))
+
+
+def test_the_largest_length_stands_for_the_whole_table():
+    cache = Cache([80, 48], [80, 80], 16, 2, 64, BF16)
+    q = normal(2, 4, 64, dtype=BF16)
+    want = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
+    assert torch.equal(fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths([2**31 - 1, 48])), want)
