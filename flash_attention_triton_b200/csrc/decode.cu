@@ -573,9 +573,8 @@ __global__ void __launch_bounds__(kJoinMost) decode_join_kernel(const __grid_con
   auto add = [&](float m, float l, float2 x, float now) {
     const float f = part_weight(m, l, now, a.scale_log2);
     all = fmaf(f, l, all);
-    // (weight 0: the part may have been left out, and hold anything)
-    sum.x = f == 0.f ? sum.x : fmaf(f, x.x, sum.x);
-    sum.y = f == 0.f ? sum.y : fmaf(f, x.y, sum.y);
+    sum.x = fmaf(f, x.x, sum.x);  // (0 x NaN is NaN in whichever part it stands)
+    sum.y = fmaf(f, x.y, sum.y);
   };
   auto lower = [&](float now) {
     const float old = part_weight(top, all, now, a.scale_log2);
@@ -598,7 +597,7 @@ __global__ void __launch_bounds__(kJoinMost) decode_join_kernel(const __grid_con
       float now = top;
 #pragma unroll
       for (int j = 0; j < kJoinBatch; ++j) {
-        if (!some[j]) ml[j] = make_float2(-INFINITY, 0.f);
+        if (!some[j]) ml[j] = make_float2(-INFINITY, 0.f), x[j] = make_float2(0.f, 0.f);  // the place may hold anything
         now = fmaxf(now, ml[j].x);
       }
       lower(now);

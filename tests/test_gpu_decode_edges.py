@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -53,3 +55,21 @@ def test_the_largest_length_stands_for_the_whole_table():
     q = normal(2, 4, 64, dtype=BF16)
     want = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths())
     assert torch.equal(fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths([2**31 - 1, 48])), want)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("where", [200, 500, 5000, 9999, 19000])
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("peak", ["front", "back"])
+def test_a_value_of_vanishing_weight_is_not_lost(peak, value, where, heads, kv_heads, d):
+    """Some keys are 200 nats above the others: 0 x NaN and 0 x infinity are NaN in whichever of the parts that are joined they stand."""
+    n, scale = 20000, 8.0 / d
+    cache = Cache([n], [n], 16, kv_heads, d, BF16)
+    q = torch.ones(1, heads, d, dtype=BF16, device="cuda")
+    k = normal(n, kv_heads, d, dtype=torch.float32) * 0.01
+    k[slice(0, 100) if peak == "front" else slice(n - 100, n)] = 25.0
+    cache.k[cache.places(0, range(n))] = k.to(BF16)
+    assert fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths(), scale).isfinite().all()
+    cache.v[cache.places(0, [where])] = value
+    out = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths(), scale)
+    assert not out.isfinite().any()
