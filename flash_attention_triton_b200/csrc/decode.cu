@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(32 * kWarps, DecodeCfg<DP, HP>::kCtasPerSm)
   uint32_t qb[HP][kSteps][NT][2];
   float o[HP][kSteps][NT][4];  // rows (columns of V) 16 i + lane / 4 (+ 8), columns (query heads) 8 t + 2 (lane % 4) (+ 1)
   float m[HP][NT][2], l[HP][NT][2];
-  const float threshold = weight_lag<BF16>(8.f) / a.scale_log2;
+  // (finite for any scale, so that a first finite score is above it)
+  const float threshold = fminf(weight_lag<BF16>(8.f) / a.scale_log2, 3e38f);
   uint32_t phases = 0;  // bit s: parity of the next wait on stage s
   bool fresh = true, ok = true;
   bool begins = work.unit == 0;  // the first unit of the (sequence, key head) is in this stretch

@@ -8,10 +8,10 @@ import pytest
 import torch
 
 from flash_attention_triton_b200 import _lib
-from paged_helpers import Cache, fa
+from paged_helpers import Cache, decode_tolerance, exact_decode, fa
 
 pytestmark = pytest.mark.gpu
-BF16 = torch.bfloat16
+BF16, FP16 = torch.bfloat16, torch.float16
 
 
 @pytest.fixture(autouse=True)
@@ -73,3 +73,14 @@ def test_a_value_of_vanishing_weight_is_not_lost(peak, value, where, heads, kv_h
     cache.v[cache.places(0, [where])] = value
     out = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths(), scale)
     assert not out.isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 1e-40])
+def test_tiny_scales(scale, dtype):
+    """All weights are alike, normal number or not."""
+    cache = Cache([300, 1, 7000], [300, 1, 7000], 16, 2, 64, dtype)
+    q = normal(3, 4, 64, dtype=dtype)
+    out = fa.flash_attention_decode(q, cache.k, cache.v, cache.table, cache.lengths(), scale)
+    want, absolute, largest = exact_decode(q, cache.keys, cache.values, scale)
+    assert ((out.double() - want).abs() <= decode_tolerance(dtype, want, absolute, largest, 64, 7000)).all()
