@@ -49,7 +49,9 @@ void check_status_if_asked(const char* fn, const at::Tensor& on) {
     pybind11::module_::import("flash_attention_triton_b200.api").attr("_check_status_if_asked")(fn, on.device());
   } catch (pybind11::error_already_set& e) {
     e.restore();
-    throw python_error();
+    python_error error;
+    error.persist();  // a backward pass may throw it on another thread
+    throw error;
   }
 }
 }  // namespace fa2_host

@@ -89,6 +89,10 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
                                 n.batch, n.Hq, n.Hkv, n.D, dtype_code(q), static_cast<float>(ctx->saved_data["scale"].toDouble()),
                                 strides.data(), stream_of(q)));
     }
+    {
+      pybind11::gil_scoped_acquire gil;
+      check_status_if_asked("fa2_packed_bwd", q);
+    }
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
