@@ -101,7 +101,7 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
   const size_t heads = static_cast<size_t>(p.capacity) * Hq;
   const PackedStats stats{static_cast<float*>(workspace), words + heads * 256, words + heads * (256 + 4)};
   const int cluster = packed_cluster(s, ctx.num_sms);
-  const int step = packed_step_rows(s, Hkv * cluster, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
+  const int step = cluster > 1 ? 128 : packed_step_rows(s, Hkv, ctx.num_sms), dq_step = packed_step_rows(s, Hq, ctx.num_sms);
   CUtensorMap tq, tk, tv, tdo, tdq, tdk, tdv;
   if (int e = tq_.map(&tq, rows, D, dtype, step)) return e;
   if (int e = tdo_.map(&tdo, rows, D, dtype, step)) return e;

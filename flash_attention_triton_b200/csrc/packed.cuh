@@ -82,7 +82,8 @@ cudaError_t launch_packed_fwd(const PackedShape& s, const int* cu_seqlens, const
 cudaError_t launch_packed_preprocess(const PackedShape& s, const PackedPlan& plan, const int* cu_seqlens, const void* o,
                                      const void* dout, const RowStrides& sdo, const float* lse, const PackedStats& stats,
                                      void* dq, void* dk, void* dv, cudaStream_t stream);
-// Rows of a step of a backward kernel with `heads` CTAs to a tile, and the box height of the tensors it walks.
+// Rows of a step of a backward kernel with `heads` CTAs to a tile, and the box height of the tensors it walks; of the dK / dV kernel in
+// clusters, which are for launches of few CTAs, 128.
 int packed_step_rows(const PackedShape& s, int heads, int num_sms);
 // CTAs of the dK / dV kernel that share the query heads of a KV tile: 1, 2 or 4, a divisor of G.
 int packed_cluster(const PackedShape& s, int num_sms);

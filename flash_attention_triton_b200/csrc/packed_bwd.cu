@@ -689,8 +689,10 @@ template <int D, bool BF16, int KD, int W>
 cudaError_t launch_dkdv_t(const PackedShape& s, const PackedPlan& plan, const CUtensorMap& tq, const CUtensorMap& tk,
                           const CUtensorMap& tv, const CUtensorMap& tdo, const CUtensorMap& tdk, const CUtensorMap& tdv,
                           void* dk, void* dv, const PackedStats& stats, int cluster, int* status, cudaStream_t stream) {
-  if (cluster == 4) return launch_dkdv_s<D, BF16, KD, W, 4>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
-  if (cluster == 2) return launch_dkdv_s<D, BF16, KD, W, 2>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
+  if constexpr (W == 128) {
+    if (cluster == 4) return launch_dkdv_s<D, BF16, KD, W, 4>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
+    if (cluster == 2) return launch_dkdv_s<D, BF16, KD, W, 2>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
+  }
   return launch_dkdv_s<D, BF16, KD, W, 1>(s, plan, tq, tk, tv, tdo, tdk, tdv, dk, dv, stats, status, stream);
 }
 template <int D, bool BF16, int KD, int W>
