@@ -69,6 +69,9 @@ __device__ __forceinline__ int sequence_of(const int* cu_seqlens, int batch, int
   return low;
 }
 
+// A sequence of a call has rows that the call has.
+__device__ __forceinline__ bool bounds_ok(int start, int end, int tokens) { return start >= 0 && start <= end && end <= tokens; }
+
 // How threads share a token's row: first those with a pair of pieces in the heads of q and k (q's heads first), then those
 // with a single piece there, then those with a piece in the heads of v.  Of the threads that have the same place, j of
 // `groups` takes heads j, j + groups, ..
@@ -109,6 +112,7 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
       // prompts 141.5 -> 138.9 us, 10 855 in 12 27.3 -> 26.2 against the search below)
       const bool there = lane < a.batch;
       const int start = there ? ld_global(a.cu_seqlens + lane) : 0, end = there ? ld_global(a.cu_seqlens + lane + 1) : 0;
+      if (blockIdx.x == 0 && !bounds_ok(start, end, a.tokens)) atomicCAS(status, 0, kStatusSequences | kSiteAppend);
       const int size = there ? ld_global(a.lengths + lane) : 0;
       // the first whose end is behind the CTA's first row, and on from there
       const unsigned behind = __ballot_sync(0xffffffffu, there && end > first);
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
       fresh = __shfl_sync(0xffffffffu, end, from) - start_of;
       length = __shfl_sync(0xffffffffu, size, from);
       index = row - start_of;
-      inside = inside && index >= 0;
+      inside = inside && index >= 0 && bounds_ok(start_of, start_of + fresh, a.tokens);
     } else {
       sequence = sequence_of(a.cu_seqlens, a.batch, first, lane);
       if (inside && sequence < a.batch && ld_global(a.cu_seqlens + sequence + 1) <= row) {  // a later sequence begins in between
@@ -141,8 +145,10 @@ __global__ void __launch_bounds__(kMostThreads, kCtasPerSm)
         length = ld_global(a.lengths + sequence);
         fresh = ld_global(a.cu_seqlens + sequence + 1) - start;
         index = row - start;
-        inside = index >= 0;
+        inside = index >= 0 && bounds_ok(start, start + fresh, a.tokens);
       }
+      for (int i = blockIdx.x * 32 + lane; i < a.batch; i += gridDim.x * 32)  // what none of these tokens sees, a share for each CTA
+        if (!bounds_ok(ld_global(a.cu_seqlens + i), ld_global(a.cu_seqlens + i + 1), a.tokens)) atomicCAS(status, 0, kStatusSequences | kSiteAppend);
     }
     TokenPlace place{-1, -1, -1};
     if (inside) {

@@ -68,9 +68,6 @@ inline size_t packed_stats_bytes(int rows, int batch, int Hq) {
   return static_cast<size_t>(packed_capacity(rows, batch)) * Hq * (256 + 4) * 4 + 16;
 }
 
-// Status word of cu_seqlens that fall, or leave the rows: every output is zero then.
-constexpr int kStatusSequences = 0x80000;
-
 cudaError_t launch_packed_plan(const PackedShape& s, const int* cu_seqlens, const PackedPlan& plan, bool pairs, void* out,
                                int* status, int num_sms, cudaStream_t stream);
 // Whether the forward has no plan kernel in front of it.  Its CTAs then find their items in cu_seqlens by themselves, and it writes the plan for

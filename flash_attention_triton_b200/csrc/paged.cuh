@@ -9,6 +9,9 @@ namespace fa2 {
 // Status word of a kernel that met a page outside the cache, or a position beyond the block table or the rotation
 // tables: what it stands for is neither read nor written.
 constexpr int kStatusPage = 0x40000;
+// Status word of cu_seqlens that fall, or leave the rows: every output of the attention is zero then; the append leaves out the tokens of
+// sequences that leave the rows.
+constexpr int kStatusSequences = 0x80000;
 enum PagedSite { kSiteAppend = 1, kSiteDecode };
 
 // Element strides; the last dimension is contiguous.

@@ -57,7 +57,8 @@ def append_kv_cache(
         block_table: int32 ``[batch, width]``.
         lengths: int32 ``[batch]``, positions in the cache once this call's tokens are in it.
         cu_seqlens: int32 ``[batch + 1]``: rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` are the last positions of
-            sequence ``s``.  ``None``: one token for each sequence.
+            sequence ``s``.  ``None``: one token for each sequence.  Tokens of a sequence that leaves the rows are left out, and the
+            status word is set; so it is where the entries fall, and which tokens are written then is not said.
         q: ``[tokens, heads, headdim]``, rotated by the same positions into a new tensor.
         cos, sin: fp32 ``[positions, rotated columns / 2]`` (:func:`rotary_tables`): the first columns of every key and
             query are rotated, the others kept.  ``None``: nothing is rotated.

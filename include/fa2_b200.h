@@ -303,7 +303,8 @@ int fa2_packed_bwd(const void* q, const void* k, const void* v, const void* o, c
  * cu_seqlens (int32 [batch + 1]) says which rows are whose: rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 are the
  * last positions of sequence s.  NULL: one token a sequence, tokens == batch.  Row i of sequence s has position
  * p = lengths[s] - (its rows) + i; a token of a negative position is not written.  Two tokens of a call must not
- * have the same slot.
+ * have the same slot.  Tokens of a sequence whose rows are not all in [0, tokens) are left out and set the status word
+ * (0x80000 | 1); so do cu_seqlens that fall, of which it is not said which tokens are written.
  * rotary: the first `rotary` columns of every key are rotated by position (0: none): columns (j, j + rotary / 2),
  * or (2 j, 2 j + 1) with `interleaved`, by the angle whose cosine and sine are cos[p][j] and sin[p][j], fp32
  * [positions, rotary / 2].  fp32 arithmetic, rounded once.
