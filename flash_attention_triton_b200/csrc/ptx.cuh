@@ -119,14 +119,16 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, co
 // and its writes are visible.  grid_allow_next lets the successor start once every CTA of this grid has
 // called it, which is after its own wait and after its tensor memory has been allocated: a successor's
 // CTA can therefore never hold the tensor memory that a CTA of this grid still needs, and when it
-// starts, everything before this grid has completed.
+// starts, everything before this grid has completed.  One kernel waits otherwise (grid_wait_unless): what starts
+// behind that one may find the grid in front of it running still, so no kernel may do without its own wait.
 // ----------------------------------------------------------------------------------------
 __device__ __forceinline__ void grid_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // For a kernel that touches nothing its predecessor reads or writes, only what kernels before that one have left.  The predecessor
 // releases a flag behind its own wait, and who acquires it has seen all that the predecessor's wait made visible, the
 // asynchronous copies' view included; without the flag (zeroed by a kernel before) the wait is the usual one.  One CTA must wait
-// for the predecessor before it ends, so that the kernel does not complete before it.
+// for the predecessor before it ends, so that the kernel does not complete before it.  Its grid_allow_next lets a successor start while
+// the predecessor still runs: two grids back is not "completed" for that one until its own grid_wait_previous has returned.
 __device__ __forceinline__ void release_flag(unsigned* flag) {
   asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
 }
