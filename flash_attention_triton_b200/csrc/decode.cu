@@ -17,7 +17,7 @@
 // movmatrix.  Eight query heads fill the product; as its rows they would fill half of it.  The four warps meet
 // where a (sequence, key head) ends, while their next stages are already loading.  The products take a fraction of
 // the time that the bytes take, so mma.sync serves, and a row of eight queries needs no tile of 128.
-// 128 sequences of 500 to 8192 keys (344 905 in all), 32 / 8 heads of 128 columns, pages of 16: 233 us, 92 % of the measured copy
+// 128 sequences of 500 to 8192 keys (344 905 in all), 32 / 8 heads of 128 columns, pages of 16: 231 to 244 us, 88 to 93 % of the measured copy
 // rate.  Two sequences of 100 000 to 131 072, 16 / 2 heads of 128, pages of 64: 53.5 us, 47 of them decode_kernel (5.6 TB/s).
 #include <algorithm>
 

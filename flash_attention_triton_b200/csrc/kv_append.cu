@@ -10,7 +10,7 @@
 // that the rotation joins in two heads, or the same piece in four.  Their loads are in flight together, and the cosines and
 // sines are read once for all of them.  Many small CTAs: one loads while others look up places or store.  The first
 // warp of a CTA finds sequence, position and page of the CTA's tokens and leaves them in shared memory.
-// 31 323 tokens of 32 + 8 + 8 heads of 128 columns: 139 us, 92 % of the measured copy rate; with one head a thread, each token
+// 31 323 tokens of 32 + 8 + 8 heads of 128 columns: 137 us, 92 % of the measured copy rate (on new inputs every call 145, 87 %); with one head a thread, each token
 // behind the stores of the one before, 183 us, with 512 threads to a CTA 178 us, five and six CTAs of 256 threads on an SM
 // (48 and 40 registers, spilled) 148 and 161 us; with the first token's loads in front of the look-up, which then waits behind
 // those of the whole SM, 184 us.

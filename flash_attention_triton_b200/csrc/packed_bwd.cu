@@ -5,11 +5,12 @@
 // that share it, one head after the other, so dK and dV are summed over them in tensor memory, in a fixed order and
 // without another pass; a CTA of the dQ kernel has one Q tile of a query head.  Both recompute the scores, so
 // no memory beyond O(rows) is needed and the same call gives the same bits.  P and dS enter the second products in 16 bits, the
-// type that the tensor pipe takes beside dO, Q and K: the gradients' error against exact ones is 1.5 times that of their own rounding.
+// type that the tensor pipe takes beside dO, Q and K: the gradients' error against exact ones is 1.4 to 1.5 times that of their own
+// rounding, up to 1.65 times on sequences of few rows, where delta has the rounding of O.
 // Bound by the tensor pipe: seven products where five would do.  bf16, 23 202 rows in three sequences, 16 / 4 heads of
 // 128 columns, each kernel alone: dK / dV 1 118 us (four products, 1 474 GFLOP, tensor pipe 74 % active), dQ 913 us (three products, 64 %);
-// in a loop under the power limit 1 245 and 1 112.  Handing dS over through memory would save two of the seven products and take
-// 8.6 GB of scratch in place of 2.9: its size is quadratic in lengths that only the device knows.
+// in a loop under the power limit 1 245 and 1 112.  Handing dS over through memory would save two of the seven products; it
+// takes scratch that is quadratic in the lengths, 8.6 GB for all 16 heads at once and 2.1 for four at a time, and a caller who says the longest.
 #include "bwd_roles.cuh"
 #include "packed.cuh"
 
