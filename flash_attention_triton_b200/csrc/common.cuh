@@ -50,6 +50,8 @@ __host__ __device__ __forceinline__ uint32_t swizzled_offset_128B(uint32_t row, 
 template <bool BF16>
 constexpr float kWeightPower = BF16 ? 0.0f : 11.0f;  // logarithm to 2
 template <bool BF16>
+constexpr float kWeightInverse = BF16 ? 1.0f : 1.0f / 2048;  // taken from the sum before its logarithm, whose error grows with it
+template <bool BF16>
 constexpr float weight_lag(float lag) { return BF16 || lag < 4.0f ? lag : 4.0f; }  // the same, of the largest factor above the running maximum
 
 // ----------------------------------------------------------------------------------------

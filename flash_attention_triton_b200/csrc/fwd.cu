@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdCfg<D == 256 ? 128 : D, W>::kC
       }
       tc_fence_before();  // O_i is overwritten by the next item's first product, which this group's P lets in
       if (row < N)
-        lse[static_cast<size_t>(item.bh) * N + row] = (m_run * scale_log2 + (lg2(l_run) - kWeightPower<BF16>)) * kLn2;
+        lse[static_cast<size_t>(item.bh) * N + row] = (m_run * scale_log2 + lg2(l_run * kWeightInverse<BF16>)) * kLn2;
     }
     if constexpr (C::kStageInQ) {
       // A group without a tile has waited for nothing yet: its arrival must not count for the item before.

@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         tc_fence_before();  // O_i is overwritten by the next item's first product, which this group's P lets in
-        if (mine) lse[static_cast<size_t>(head) * rows + row] = (m_run * scale_log2 + (lg2(l_run) - kWeightPower<BF16>)) * kLn2;
+        if (mine) lse[static_cast<size_t>(head) * rows + row] = (m_run * scale_log2 + lg2(l_run * kWeightInverse<BF16>)) * kLn2;
       }
     }  // items
     if (lane == 0) tma_store_wait_read();
